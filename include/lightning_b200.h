@@ -262,6 +262,45 @@ int lab200_srmsnorm_gate_fwd(const void* x, const void* gate, void* y, float* rs
 int lab200_srmsnorm_gate_bwd(const void* x, const void* gate, const void* dy, const float* rstd, void* dx,
                              void* dgate, long long M, int N, int dtype, void* stream);
 
+/*
+ * Layer norm with weight and bias over the last dimension, alone or followed by a sigmoid gate (what the reference's example
+ * caller does with nn.LayerNorm, examples/module/tnl_attn.py:66-69):
+ *   xh = (x - mean) * rstd;  n = xh * weight + bias;  y = n, or n * sigmoid(gate)
+ * x, gate: M rows of N elements of `dtype`, ldx / ldg elements from one row to the next (>= N, ignored for a single row); gate may
+ * be NULL. weight, bias: N values of `wdtype` (dtype or LAB200_F32), or NULL for ones / zeros. y: (M, N) contiguous.
+ * stats: (M, 2) fp32, mean and rstd of each row for the backward pass, 8-byte aligned, or NULL.
+ * xcodes, xscales (and gcodes, gscales with a gate): NULL, or where the 8-bit checkpoints of x (and gate) go, laid out as
+ * lab200_pack8 writes them. Any N up to 2^30; eps >= 0.
+ */
+int lab200_layernorm_fwd(const void* x, long long ldx, const void* gate, long long ldg, const void* weight, const void* bias,
+                         int wdtype, void* y, float* stats, void* xcodes, void* xscales, void* gcodes, void* gscales, long long M,
+                         int N, float eps, int dtype, void* stream);
+
+/* Bytes of workspace lab200_layernorm_bwd needs for the gradients of weight and bias (0 without them). */
+size_t lab200_layernorm_bwd_workspace_bytes(long long M, int N);
+
+/*
+ * Gradients of the above. x (and gate) are given as tensors, or, with x (and gate) NULL, as the checkpoints that the forward pass
+ * wrote. dy: rows of lddy; dx, dgate: (M, N) contiguous of `dtype`; dweight, dbias: N values of `wdtype`. Each of the four may
+ * be NULL where it is not wanted. bias only matters with a gate. Deterministic: sums over rows go through partial sums in
+ * `workspace` (16-byte aligned) in a fixed order.
+ */
+int lab200_layernorm_bwd(const void* x, long long ldx, const void* gate, long long ldg, const void* xcodes, const void* xscales,
+                         const void* gcodes, const void* gscales, const float* stats, const void* dy, long long lddy,
+                         const void* weight, const void* bias, int wdtype, void* dx, void* dgate, void* dweight, void* dbias,
+                         void* workspace, size_t workspace_bytes, long long M, int N, int dtype, void* stream);
+
+/*
+ * 8-bit checkpoint of M rows of N values (row stride ldx): each 32 consecutive values of a row, the last of a row fewer, share
+ * an exponent byte E and keep a signed byte each, value = code * 2^(E - 133), off by at most half of that step; E = 255: the
+ * group held an infinity or a NaN and comes back as NaN. codes: (M, N) int8; scales: (M, ceil(N / 32)) uint8, both contiguous.
+ * Rounding is to nearest even and exact whatever the type of x. No counterpart in the reference.
+ */
+int lab200_pack8(const void* x, long long ldx, void* codes, void* scales, long long M, int N, int dtype, void* stream);
+
+/* The values that a checkpoint stands for, (M, N) contiguous of `dtype` (fp16: kept within +-65504). */
+int lab200_unpack8(const void* codes, const void* scales, void* y, long long M, int N, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -77,6 +77,16 @@ def lib():
         L.lab200_srmsnorm_fwd.argtypes = [vp, vp, vp, ll, i, f, i, vp]
         L.lab200_srmsnorm_bwd.restype = i
         L.lab200_srmsnorm_bwd.argtypes = [vp, vp, vp, vp, ll, i, i, vp]
+        L.lab200_layernorm_fwd.restype = i
+        L.lab200_layernorm_fwd.argtypes = [vp, ll, vp, ll, vp, vp, i, vp, vp, vp, vp, vp, vp, ll, i, f, i, vp]
+        L.lab200_layernorm_bwd_workspace_bytes.restype = sz
+        L.lab200_layernorm_bwd_workspace_bytes.argtypes = [ll, i]
+        L.lab200_layernorm_bwd.restype = i
+        L.lab200_layernorm_bwd.argtypes = [vp, ll, vp, ll, vp, vp, vp, vp, vp, vp, ll, vp, vp, i, vp, vp, vp, vp, vp, sz, ll, i, i, vp]
+        L.lab200_pack8.restype = i
+        L.lab200_pack8.argtypes = [vp, ll, vp, vp, ll, i, i, vp]
+        L.lab200_unpack8.restype = i
+        L.lab200_unpack8.argtypes = [vp, vp, vp, ll, i, i, vp]
         _lib = L
     return _lib
 
@@ -142,6 +152,7 @@ EXPORTS = [
     "lab200_version", "lab200_launch_count", "lab200_la_debug_trace", "lab200_error_string", "lab200_la_plan_chunks", "lab200_la_workspace_bytes",
     "lab200_la_generic", "lab200_la_generic_resume", "lab200_la_generic_resume_swapped", "lab200_la_combine_states", "lab200_la_decode_step", "lab200_la2_fwd", "lab200_la2_fwd_static", "lab200_la2_bwd", "lab200_la2_bwd_workspace_bytes", "lab200_la2_bwd_kept", "lab200_la2_dkdv", "lab200_read_status", "lab200_last_status", "lab200_static_status", "lab200_debug_wait_expiry",
     "lab200_srmsnorm_fwd", "lab200_srmsnorm_bwd", "lab200_srmsnorm_gate_fwd", "lab200_srmsnorm_gate_bwd",
+    "lab200_layernorm_fwd", "lab200_layernorm_bwd", "lab200_layernorm_bwd_workspace_bytes", "lab200_pack8", "lab200_unpack8",
 ]
 
 

@@ -17,14 +17,14 @@ else:  # run by its path
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_NAME = "liblightning_b200.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
-SOURCES = [os.path.join(HERE, "csrc", "capi.cu")]
+SOURCES = [os.path.join(HERE, "csrc", "capi.cu"), os.path.join(HERE, "csrc", "norm_api.cu")]
 import glob
 
-HEADERS = sorted(glob.glob(os.path.join(HERE, "csrc", "*.cuh"))) + [os.path.join(HERE, "..", "include", "lightning_b200.h")]
+HEADERS = sorted(glob.glob(os.path.join(HERE, "csrc", "*.cuh")) + glob.glob(os.path.join(HERE, "csrc", "*.h"))) + [os.path.join(HERE, "..", "include", "lightning_b200.h")]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
-    "-shared", "-Xcompiler", "-fPIC",
+    "-Xcompiler", "-fPIC",
 ]
 
 
@@ -58,6 +58,22 @@ def _run(cmd, what, verbose):
         raise RuntimeError(f"{what} failed:\n" + res.stdout + res.stderr)
 
 
+def build_library(force=False, verbose=False):
+    """Compile each of SOURCES that is older than itself or a header to an object file beside it, all at once, and link them."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    nvcc = find_nvcc()
+    objects = [os.path.splitext(src)[0] + ".o" for src in SOURCES]
+
+    def compile_one(src, obj):
+        _run([nvcc] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-c", "-o", obj, src], "nvcc", verbose)
+
+    todo = [(src, obj) for src, obj in zip(SOURCES, objects) if force or not _newer(obj, [src] + HEADERS)]
+    with ThreadPoolExecutor(max(1, len(todo))) as pool:
+        list(pool.map(lambda t: compile_one(*t), todo))
+    _run([nvcc] + NVCC_FLAGS + ["-shared", "-o", LIB_PATH] + objects, "nvcc", verbose)
+
+
 def build_host(verbose=False):
     """Compile _host_ops.so against the torch this interpreter imports."""
     import sysconfig
@@ -78,7 +94,7 @@ def build_host(verbose=False):
 def build(force=False, verbose=False):
     """Compile what is missing or older than its sources. Returns the path of the C-ABI library."""
     if force or not _newer(LIB_PATH, SOURCES + HEADERS):
-        _run([find_nvcc()] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-o", LIB_PATH] + SOURCES, "nvcc", verbose)
+        build_library(force, verbose)
     if force or not _newer(HOST_PATH, HOST_SOURCES) or _lib.host_built_for(HOST_PATH) != _lib.host_abi():
         build_host(verbose)
     return LIB_PATH

@@ -10,6 +10,7 @@
 #include <mutex>
 
 #include "../../include/lightning_b200.h"
+#include "launch_count.h"
 #include "la_kernels.cuh"
 #include "la_pipe_kernel.cuh"
 #include "la_dkdv2_kernel.cuh"
@@ -685,6 +686,8 @@ __global__ void la_wait_expiry_kernel(LaStatus status, long long budget) {
 }
 
 }  // namespace
+
+void lab200::count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
 
 extern "C" {
 

@@ -12,6 +12,7 @@ C-ABI calls without Python in between), which answers None to every call that is
 import torch
 
 from ... import _lib
+from .checkpoint8 import checkpoint_fits, differentiable_once, pack_8bit, unpack_8bit
 
 
 def _slopes_arg(s, h, device):
@@ -324,6 +325,37 @@ class LightningAttention2NoDecay(torch.autograd.Function):
         return _bwd(q, k, v, None, do, bnhd=ctx.bnhd, kept=kept)
 
 
+class LightningAttention2Saved8(torch.autograd.Function):
+    """The same with q, k, v kept for the backward pass as 8-bit checkpoints (checkpoint8.py); s None: no decay. The forward pass is that
+    of the classes above; the gradients are theirs at the checkpoints' values, chunk states included, which are computed from those."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, s):
+        _check_inputs(q, k, v)
+        bnhd = _use_bnhd(q, k, v)
+        q, k, v = (_to_layout(t, bnhd) for t in (q, k, v))
+        s = None if s is None else s.contiguous()
+        o = _fwd(q, k, v, _slopes_arg(s, q.shape[1], q.device), bnhd=bnhd)
+        # in the order of the memory, so that groups of 32 lie in one token's features
+        packed = [pack_8bit(t.transpose(1, 2) if bnhd else t) for t in (q, k, v)]
+        ctx.save_for_backward(s, *(p for pair in packed for p in pair))
+        ctx.info = (q.dtype, bnhd, [tuple(p[0].shape) for p in packed])
+        return o
+
+    @staticmethod
+    def backward(ctx, do):
+        differentiable_once("lightning attention with save_8bit")
+        dtype, bnhd, shapes = ctx.info
+        s, *packed = ctx.saved_tensors
+        pairs = list(zip(packed[0::2], packed[1::2]))
+        if not all(checkpoint_fits(c, sc, shape, do.device) for (c, sc), shape in zip(pairs, shapes)):
+            raise RuntimeError("lightning attention backward: saved-tensor hooks returned another shape, dtype or device")
+        q, k, v = (unpack_8bit(c, sc, dtype) for c, sc in pairs)
+        if bnhd:
+            q, k, v = (t.transpose(1, 2) for t in (q, k, v))
+        return _bwd(q, k, v, _slopes_arg(s, q.shape[1], q.device), _to_layout(do, bnhd), bnhd=bnhd) + (None,)
+
+
 def lightning_attn_prefill(q, k, v, s=None, kv_state=None):
     """Forward pass that carries the recurrence state, for inference (no autograd; the reference has no such entry).
 
@@ -374,8 +406,15 @@ def lightning_attn_decode(q, k, v, s, kv_state):
     return o.unsqueeze(2) if squeeze else o
 
 
-def lightning_attn2(q, k, v, s):
-    """LightningAttention2 through the native call path where the call has the common form, else through the class."""
+def _backward_can_follow(*tensors):
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+
+
+def lightning_attn2(q, k, v, s, save_8bit=False):
+    """LightningAttention2 through the native call path where the call has the common form, else through the class. save_8bit: the
+    backward pass keeps q, k, v as 8-bit checkpoints (`pack_8bit`) and gives the gradients at their values."""
+    if save_8bit and _backward_can_follow(q, k, v):
+        return LightningAttention2Saved8.apply(q, k, v, s)
     if s is not None and not torch.compiler.is_compiling():
         o = _lib.host().attn(q, k, v, s)
         if o is not None:
@@ -383,8 +422,10 @@ def lightning_attn2(q, k, v, s):
     return LightningAttention2.apply(q, k, v, s)
 
 
-def lightning_attn2_no_decay(q, k, v):
+def lightning_attn2_no_decay(q, k, v, save_8bit=False):
     """LightningAttention2NoDecay, the same way."""
+    if save_8bit and _backward_can_follow(q, k, v):
+        return LightningAttention2Saved8.apply(q, k, v, None)
     if not torch.compiler.is_compiling():
         o = _lib.host().attn_no_decay(q, k, v)
         if o is not None:

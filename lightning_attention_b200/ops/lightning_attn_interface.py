@@ -31,23 +31,24 @@ def _pad_last(x, mult):
     return F.pad(x, (0, r)) if r else x
 
 
-def lightning_attn_func(q, k, v, s=None, variant="chunk_loop"):
+def lightning_attn_func(q, k, v, s=None, variant="chunk_loop", save_8bit=False):
     """o_t = sum_{j<=t} exp(-s (t-j)) (q_t . k_j) v_j per head; s=None means no decay.
 
-    `variant` is accepted for compatibility ("chunk_loop" or "parallel"); one implementation serves both.
+    `variant` is accepted for compatibility ("chunk_loop" or "parallel"); one implementation serves both. save_8bit: q, k, v are
+    kept for the backward pass in 8 bits (`pack_8bit`: 8.25 bits per value in place of 16), which then gives the gradients at those values.
     """
     if variant not in ("chunk_loop", "parallel"):
         raise ValueError(f"unknown variant {variant!r}")
     d, e = q.shape[-1], v.shape[-1]
     if d % 16 == 0 and e % 16 == 0 and k.shape[-1] == d and d <= _MAX_D and e <= _MAX_D:
-        return lightning_attn2_no_decay(q, k, v) if s is None else lightning_attn2(q, k, v, s)
+        return lightning_attn2_no_decay(q, k, v, save_8bit) if s is None else lightning_attn2(q, k, v, s, save_8bit)
     q = _pad_last(q, 16)
     k = _pad_last(k, 16)
     v = _pad_last(v, 16)
     d = q.shape[-1]
 
     def fn(q1, k1, v1):
-        return lightning_attn2_no_decay(q1, k1, v1) if s is None else lightning_attn2(q1, k1, v1, s)
+        return lightning_attn2_no_decay(q1, k1, v1, save_8bit) if s is None else lightning_attn2(q1, k1, v1, s, save_8bit)
 
     def over_d(v1):
         # q.k is additive over feature slices and the output is linear in it: d > 256 runs as slices whose partial outputs are
