@@ -17,7 +17,7 @@ else:  # run by its path
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_NAME = "liblightning_b200.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
-SOURCES = [os.path.join(HERE, "csrc", "capi.cu"), os.path.join(HERE, "csrc", "norm_api.cu")]
+SOURCES = [os.path.join(HERE, "csrc", name) for name in ("capi.cu", "norm_api.cu", "layernorm_f32.cu", "layernorm_f16.cu", "layernorm_bf16.cu")]
 import glob
 
 HEADERS = sorted(glob.glob(os.path.join(HERE, "csrc", "*.cuh")) + glob.glob(os.path.join(HERE, "csrc", "*.h"))) + [os.path.join(HERE, "..", "include", "lightning_b200.h")]

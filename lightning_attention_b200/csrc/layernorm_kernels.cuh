@@ -21,6 +21,7 @@ struct LnArgs {
   uint8_t *xscales, *gscales;
   const void *weight, *bias;     // NULL: ones, zeros
   int wdt;                       // their type
+  bool vec_params;               // and whether they may be read 16 bytes at a time
   void* y;
   float2* stats;                 // (m, r) of each row; forward: NULL where nobody wants them
   const void* dy;
@@ -198,28 +199,512 @@ __global__ void __launch_bounds__(256) ln_bwd_columns_kernel(const LnArgs a) {
   }
 }
 
-// dw and db from their parts: a CTA per 32 columns, its eight warps take every eighth part. No part: zeros.
-__global__ void __launch_bounds__(256) ln_bwd_join_kernel(const float* __restrict__ partial, int nparts, int N, void* dw, void* db, int wdt) {
-  __shared__ float red[2][8][32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (long long c0 = static_cast<long long>(blockIdx.x) * 32; c0 < N; c0 += static_cast<long long>(gridDim.x) * 32) {
-    const int col = static_cast<int>(c0) + lane;
-    const bool on = lane < N - c0;
-    float s[2] = {0.f, 0.f};
-    for (int p = warp; on && p < nparts; p += 8) {
-      s[0] += partial[(static_cast<size_t>(p) * 2) * N + col];
-      s[1] += partial[(static_cast<size_t>(p) * 2 + 1) * N + col];
-    }
-    red[0][warp][lane] = s[0];
-    red[1][warp][lane] = s[1];
-    __syncthreads();
-    if (warp < 2 && on) {
-      float v = 0.f;
+// ---- rows that packs of 16 bytes divide ------------------------------------------------------------------------------------
+// A pack is P = 8 (16-bit) or 4 (fp32) values. Copies into shared memory run ahead (cp.async), every value comes from memory once in
+// each pass, and CTAs walk over the rows with what belongs to the columns at hand.
+
+// Two fp32 values in one 64-bit register: the packed arithmetic of sm_100 does both at once.
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 f2_of(float lo, float hi) { f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi)); return r; }
+__device__ __forceinline__ f2 f2_all(float v) { return f2_of(v, v); }
+__device__ __forceinline__ float2 f2_get(f2 v) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v)); return r; }
+__device__ __forceinline__ f2 f2_add(f2 a, f2 b) { f2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f2 f2_mul(f2 a, f2 b) { f2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f2 f2_fma(f2 a, f2 b, f2 c) { f2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ float f2_sum(f2 v) { const float2 t = f2_get(v); return t.x + t.y; }
+
+// Copies of 4, 8 or 16 bytes into shared memory that the thread does not wait for; `n` of them are read, the rest becomes zero.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from, int n = BYTES) {
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(n) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(BYTES), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Waits until at most `stages` - 2 of the thread's groups are under way.
+__device__ __forceinline__ void copies_wait(int stages) {
+  if (stages == 2) asm volatile("cp.async.wait_group 0;" ::: "memory");
+  else if (stages == 3) asm volatile("cp.async.wait_group 1;" ::: "memory");
+  else asm volatile("cp.async.wait_group 2;" ::: "memory");
+}
+__device__ __forceinline__ uint4 shared16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 shared_f4(uint32_t at) {
+  const uint4 v = shared16(at);
+  return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+}
+__device__ __forceinline__ float2 shared_f2(uint32_t at) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void shared_put(uint32_t at, float2 v) { asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(v.x), "f"(v.y) : "memory"); }
+__device__ __forceinline__ void shared_put(uint32_t at, float4 v) {
+  asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+
+template <int DT>
+struct LnPack {
+  static constexpr int ESZ = DT == SRMS_F32 ? 4 : 2, P = 16 / ESZ, H = P / 2;
+  static constexpr int LANES = PK_GROUP / P;  // adjacent packs that hold one group of a checkpoint
+  using T = typename SrmsElem<DT>::T;
+
+  __device__ static void unpack(const uint4& raw, f2* out) {
+    float f[P];
+    SrmsVec<DT>::unpack(raw, f);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v += red[warp][k][lane];
-      ln_param_out(warp ? db : dw, wdt, col, v);
+    for (int j = 0; j < H; ++j) out[j] = f2_of(f[2 * j], f[2 * j + 1]);
+  }
+  __device__ static void floats(const f2* v, float* f) {
+#pragma unroll
+    for (int j = 0; j < H; ++j) {
+      const float2 t = f2_get(v[j]);
+      f[2 * j] = t.x; f[2 * j + 1] = t.y;
+    }
+  }
+  __device__ static void store(void* to, const f2* in) {
+    float f[P];
+    floats(in, f);
+    SrmsPack<1> o;
+    o.q[0] = SrmsVec<DT>::pack(f);
+    st_stream<1>(static_cast<SrmsPack<1>*>(to), o);
+  }
+  // P values of weight or bias (`p` NULL: `without`), whatever their type and alignment.
+  __device__ static void params(const void* p, int wdt, bool vec, int k, float without, float* f) {
+#pragma unroll
+    for (int e = 0; e < P; ++e) f[e] = without;
+    if (!p) return;
+    if (!vec) {
+#pragma unroll
+      for (int e = 0; e < P; ++e) f[e] = ln_param(p, wdt, k * P + e, without);
+    } else if (wdt == SRMS_F32) {
+#pragma unroll
+      for (int e = 0; e < P; e += 4) *reinterpret_cast<float4*>(f + e) = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + k * P + e));
+    } else if constexpr (DT != SRMS_F32) {
+      SrmsVec<DT>::unpack(__ldg(static_cast<const uint4*>(p) + k), f);
+    }
+  }
+  // The checkpoint of pack k of a row, whose group LANES adjacent lanes hold; all lanes of a warp call it, `on`: there is such a pack.
+  __device__ static void quantise(const f2* x, int8_t* codes, uint8_t* scales, int k, bool on) {
+    float f[P];
+    floats(x, f);
+    const uint32_t ex = pk_exponent(pk_group_max<LANES>(pk_abs_max<P>(f)));
+    uint32_t w[P / 4];
+    pk_codes<P>(f, ex, w);
+    if (on) {
+      if constexpr (P == 8) reinterpret_cast<uint2*>(codes)[k] = make_uint2(w[0], w[1]);
+      else reinterpret_cast<uint32_t*>(codes)[k] = w[0];
+      if (k % LANES == 0) scales[k / LANES] = static_cast<uint8_t>(ex);
+    }
+  }
+  // P fp32 values for each pack, in planes of four: what adjacent lanes read lies next to each other.
+  __device__ static void plane_put(uint32_t plane, int npack, int k, const float* f) {
+#pragma unroll
+    for (int e = 0; e < P; e += 4) shared_put(plane + (e / 4 * npack + k) * 16, make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]));
+  }
+  __device__ static void plane_get(uint32_t plane, int npack, int k, f2* out) {
+#pragma unroll
+    for (int e = 0; e < P; e += 4) {
+      const float4 v = shared_f4(plane + (e / 4 * npack + k) * 16);
+      out[e / 2] = f2_of(v.x, v.y);
+      out[e / 2 + 1] = f2_of(v.z, v.w);
+    }
+  }
+};
+
+extern __shared__ __align__(16) char ln_shared[];
+
+// ---- forward -----------------------------------------------------------------------------------------------------------------
+// A row is a team's of T threads, V packs a thread: T a power of two up to 32 (several rows in a warp) or a multiple of 32. A warp
+// has the mean and the squares about it of its part of a row from shuffles; the parts are joined by the formula for the variance of
+// a union, behind the only barrier of a row. Each thread has places of its own in the ring of copies, so that it needs none.
+struct LnFwdPlan { int T, stages; };
+
+template <int DT, int V, int G, bool GATE, bool SAVE>
+__global__ void __launch_bounds__(512) ln_fwd_kernel(const LnArgs a, const LnFwdPlan plan) {
+  using K = LnPack<DT>;
+  constexpr int P = K::P, H = K::H;
+  __shared__ float4 slot[G > 32 ? 2 : 1][16];  // of a CTA's warps: mean, squares, count of their part; two halves in turn
+  const int T = G <= 32 ? G : plan.T, team = threadIdx.x / T, t = threadIdx.x - team * T, lanes = blockDim.x, warp = threadIdx.x >> 5;
+  const int N = a.N, npack = N / P, ng = (N - 1) / PK_GROUP + 1, teams = lanes / T;
+  const uint32_t wplane = static_cast<uint32_t>(__cvta_generic_to_shared(ln_shared)), bplane = wplane + N * 4, ring = bplane + N * 4 + threadIdx.x * 16;
+  const uint32_t pitch = lanes * 16, stage_bytes = pitch * V * (GATE ? 2 : 1), ring_end = plan.stages * stage_bytes;
+  const long long step = static_cast<long long>(gridDim.x) * teams;
+  long long row = static_cast<long long>(blockIdx.x) * teams + team, ahead = row;
+  long long first = G < 32 ? static_cast<long long>(blockIdx.x) * teams + (threadIdx.x & ~31) / T : row;
+  const char *x_from = static_cast<const char*>(a.x) + row * a.ldx * K::ESZ + t * 16, *g_from = static_cast<const char*>(a.gate) + row * a.ldg * K::ESZ + t * 16;
+  const long long x_step = step * a.ldx * K::ESZ, g_step = step * a.ldg * K::ESZ;
+  uint32_t in = 0, out = 0;
+  const auto start = [&] {
+    if (ahead < a.M) {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (t + i * T < npack) {
+          copy_async<16>(ring + in + i * pitch, x_from + i * T * 16);
+          if constexpr (GATE) copy_async<16>(ring + in + (V + i) * pitch, g_from + i * T * 16);
+        }
+    }
+    copies_commit();
+    ahead += step;
+    x_from += x_step;
+    g_from += g_step;
+    in = in + stage_bytes == ring_end ? 0 : in + stage_bytes;
+  };
+  for (int k = 1; k < plan.stages; ++k) start();
+  for (int k = threadIdx.x; k < npack; k += lanes) {
+    float f[P];
+    K::params(a.weight, a.wdt, a.vec_params, k, 1.f, f);
+    K::plane_put(wplane, npack, k, f);
+    K::params(a.bias, a.wdt, a.vec_params, k, 0.f, f);
+    K::plane_put(bplane, npack, k, f);
+  }
+  __syncthreads();
+  int count = 0;  // values of a row that this warp (or sub-warp team) has
+#pragma unroll
+  for (int i = 0; i < V; ++i) count += P * min(max(npack - i * T - (G < 32 ? 0 : (t & ~31)), 0), G < 32 ? G : 32);
+  const float fcount = static_cast<float>(count), inv_count = count ? 1.f / fcount : 0.f, inv_n = 1.f / static_cast<float>(N);
+  int turn = 0;
+  char* y = static_cast<char*>(a.y) + row * N * K::ESZ + t * 16;
+  const long long y_step = step * N * K::ESZ;
+  for (; first < a.M; first += step, row += step, y += y_step) {
+    const bool live = G >= 32 || row < a.M;
+    copies_wait(plan.stages);
+    uint4 raw[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) raw[i] = live && t + i * T < npack ? shared16(ring + out + i * pitch) : make_uint4(0, 0, 0, 0);
+    const uint32_t gates = ring + out + V * pitch;
+    out = out + stage_bytes == ring_end ? 0 : out + stage_bytes;
+    start();
+    f2 v[V][H];
+    f2 s = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      K::unpack(raw[i], v[i]);
+      f2 part = v[i][0];
+#pragma unroll
+      for (int j = 1; j < H; ++j) part = f2_add(part, v[i][j]);
+      s = f2_add(s, part);
+      if constexpr (SAVE) K::quantise(v[i], a.xcodes + row * N, a.xscales + row * ng, t + i * T, live && t + i * T < npack);
+    }
+    float m = f2_sum(s);
+#pragma unroll
+    for (int o = (G < 32 ? G : 32) / 2; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
+    m *= inv_count;
+    const f2 minus_m = f2_all(-m);
+    f2 d1 = 0, d2 = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      f2 p1 = 0, p2 = 0;
+#pragma unroll
+      for (int j = 0; j < H; ++j) {
+        v[i][j] = f2_add(v[i][j], minus_m);
+        p1 = f2_add(p1, v[i][j]);
+        p2 = f2_fma(v[i][j], v[i][j], p2);
+      }
+      if (t + i * T < npack) {  // packs behind the row's end take no part
+        d1 = f2_add(d1, p1);
+        d2 = f2_add(d2, p2);
+      }
+    }
+    float q1 = f2_sum(d1), q2 = f2_sum(d2);
+#pragma unroll
+    for (int o = (G < 32 ? G : 32) / 2; o > 0; o >>= 1) {
+      q1 += __shfl_xor_sync(0xffffffffu, q1, o);
+      q2 += __shfl_xor_sync(0xffffffffu, q2, o);
+    }
+    // what the warp's mean was off by, and the squares about the corrected one
+    float mean = q1 * inv_count;  // counted from m
+    float squares = fmaf(-mean, q1, q2);
+    if constexpr (G > 32) {
+      if ((t & 31) == 0) slot[turn][warp] = make_float4(m + mean, squares, fcount, 0.f);
+      asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(T) : "memory");
+      const float4* part = slot[turn] + team * (T / 32);
+      float total = 0.f, both = 0.f;
+      for (int w = 0; w < T / 32; ++w) {
+        const float d = part[w].x - m;
+        total = fmaf(part[w].z, d, total);
+        both += fmaf(part[w].z * d, d, part[w].y);
+      }
+      mean = total * inv_n;
+      squares = fmaf(-mean, total, both);
+      turn ^= 1;
+    }
+    squares *= inv_n;
+    const float r = 1.f / sqrtf((squares < 0.f ? 0.f : squares) + a.eps);
+    if (a.stats && t == 0 && live) a.stats[row] = make_float2(m + mean, r);
+    const f2 off = f2_all(-mean * r), rr = f2_all(r);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int k = t + i * T;
+      const bool on = live && k < npack;
+      f2 u[H];
+      if constexpr (GATE) {
+        K::unpack(on ? shared16(gates + i * pitch) : make_uint4(0, 0, 0, 0), u);
+        if constexpr (SAVE) K::quantise(u, a.gcodes + row * N, a.gscales + row * ng, k, on);
+      }
+      if (on) {
+        f2 w[H], b[H];
+        K::plane_get(wplane, npack, k, w);
+        K::plane_get(bplane, npack, k, b);
+#pragma unroll
+        for (int j = 0; j < H; ++j) {
+          v[i][j] = f2_fma(f2_fma(v[i][j], rr, off), w[j], b[j]);
+          if constexpr (GATE) {
+            const float2 gv = f2_get(u[j]);
+            float s0, s1, rest;
+            ln_sigmoid(gv.x, &s0, &rest);
+            ln_sigmoid(gv.y, &s1, &rest);
+            v[i][j] = f2_mul(v[i][j], f2_of(s0, s1));
+          }
+        }
+        K::store(y + i * T * 16, v[i]);
+      }
+    }
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+// ---- backward ----------------------------------------------------------------------------------------------------------------
+// A CTA takes tiles of rows into shared memory and goes over each twice. First warps (or parts of a warp) sum u and u xh over rows,
+// many values of a row to a lane, so that shuffles are few. Behind a barrier every thread has the same VP packs of columns of a number of
+// rows, which are independent of each other: dx and dgate go out, and dw and db are summed in registers.
+struct LnBwdPlan {
+  int ct, rg, rows;    // second pass: threads to a row, rows side by side, rows of a tile
+  int lanes, warps;    // first pass: lanes to a row (a power of two up to 32), warps to a row
+  int stages;
+  uint32_t dy_at, x_at, g_at, st_at, xs_at, gs_at, stage_bytes;  // within a stage
+};
+
+// The exponents of a tile's rows, which lie next to each other in memory, in whole words.
+__device__ __forceinline__ void ln_scales_async(uint32_t to, const uint8_t* from, long long lo, long long hi) {
+  for (long long w = (lo & ~3ll) + 4 * static_cast<long long>(threadIdx.x); w < hi; w += 4 * blockDim.x)
+    copy_async<4>(to + static_cast<uint32_t>(w - (lo & ~3ll)), from + w, hi - w < 4 ? static_cast<int>(hi - w) : 4);
+}
+
+// A pack of x or gate in the backward pass, from its tile in shared memory: the tensor's values, or the checkpoint's.
+template <int DT, bool SAVED>
+__device__ __forceinline__ void ln_tile_get(uint32_t packs, uint32_t exps, int row, int k, int npack, int ng, f2* out) {
+  using K = LnPack<DT>;
+  if constexpr (!SAVED) {
+    K::unpack(shared16(packs + (row * npack + k) * 16), out);
+  } else {
+    uint32_t w[K::P / 4], e;
+    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(e) : "r"(exps + row * ng + k / K::LANES) : "memory");
+    if constexpr (K::P == 8) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(packs + (row * npack + k) * 8) : "memory");
+    else asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(packs + (row * npack + k) * 4) : "memory");
+    const f2 unit = f2_all(pk_step(e));
+#pragma unroll
+    for (int c = 0; c < K::P; c += 2) out[c / 2] = f2_mul(pk_two(w[c / 4], c % 4), unit);
+  }
+}
+
+template <int DT, int VP, bool GATE, bool SAVED>
+__global__ void __launch_bounds__(VP == 1 ? 640 : 512) ln_bwd_kernel(const LnArgs a, const LnBwdPlan plan) {
+  using K = LnPack<DT>;
+  constexpr int P = K::P, H = K::H, XP = SAVED ? P : 16;
+  constexpr int V1 = 4;  // packs that a lane sums at a time in the first pass
+  const int N = a.N, npack = N / P, ng = (N - 1) / PK_GROUP + 1, tid = threadIdx.x;
+  const float inv_n = 1.f / static_cast<float>(N);
+  const uint32_t wplane = static_cast<uint32_t>(__cvta_generic_to_shared(ln_shared)), sums = wplane + N * 4, ring = sums + ((plan.rows * plan.warps * 8 + 15) & ~15);
+  const uint32_t ring_end = plan.stages * plan.stage_bytes;
+  // this thread's columns and first row in the second pass; `mine` is false for threads that are left over
+  const int rg = tid / plan.ct, c = tid - rg * plan.ct;
+  const bool mine = rg < plan.rg;
+  const long long tile_step = static_cast<long long>(gridDim.x) * plan.rows;
+  long long row0 = static_cast<long long>(blockIdx.x) * plan.rows, ahead = row0;
+  uint32_t in = 0, out = 0;
+  const auto start = [&] {
+    if (ahead < a.M) {
+      const int rows = static_cast<int>(min(static_cast<long long>(plan.rows), a.M - ahead));
+      const uint32_t st = ring + in;
+      if (mine) {
+        const char* dy = static_cast<const char*>(a.dy) + (ahead + rg) * a.lddy * K::ESZ;
+        const long long xpitch = SAVED ? N : a.ldx * K::ESZ, gpitch = SAVED ? N : a.ldg * K::ESZ;
+        const char* x = (SAVED ? reinterpret_cast<const char*>(a.xcodes) : static_cast<const char*>(a.x)) + (ahead + rg) * xpitch;
+        const char* g = (SAVED ? reinterpret_cast<const char*>(a.gcodes) : static_cast<const char*>(a.gate)) + (ahead + rg) * gpitch;
+        for (int r = rg; r < rows; r += plan.rg) {
+#pragma unroll
+          for (int i = 0; i < VP; ++i) {
+            const int k = c + i * plan.ct;
+            if (VP == 1 || k < npack) {
+              copy_async<16>(st + plan.dy_at + (r * npack + k) * 16, dy + k * 16);
+              copy_async<XP>(st + plan.x_at + (r * npack + k) * XP, x + k * XP);
+              if constexpr (GATE) copy_async<XP>(st + plan.g_at + (r * npack + k) * XP, g + k * XP);
+            }
+          }
+          dy += plan.rg * a.lddy * K::ESZ;
+          x += plan.rg * xpitch;
+          if constexpr (GATE) g += plan.rg * gpitch;
+        }
+      }
+      for (int r = tid; r < rows; r += blockDim.x) copy_async<8>(st + plan.st_at + r * 8, a.stats + ahead + r);
+      if constexpr (SAVED) {
+        ln_scales_async(st + plan.xs_at, a.xscales, ahead * ng, (ahead + rows) * ng);
+        if constexpr (GATE) ln_scales_async(st + plan.gs_at, a.gscales, ahead * ng, (ahead + rows) * ng);
+      }
+    }
+    copies_commit();
+    ahead += tile_step;
+    in = in + plan.stage_bytes == ring_end ? 0 : in + plan.stage_bytes;
+  };
+  for (int k = 1; k < plan.stages; ++k) start();
+  f2 w[VP][H], b[GATE ? VP : 1][H], dw[VP][H], db[VP][H];
+#pragma unroll
+  for (int i = 0; i < VP; ++i) {
+    const int k = c + i * plan.ct;
+    float f[P];
+    const bool on = mine && k < npack;
+    K::params(on ? a.weight : nullptr, a.wdt, a.vec_params, k, 1.f, f);
+    if (on && rg == 0) K::plane_put(wplane, npack, k, f);
+#pragma unroll
+    for (int j = 0; j < H; ++j) w[i][j] = f2_of(f[2 * j], f[2 * j + 1]);
+    if constexpr (GATE) {
+      K::params(on ? a.bias : nullptr, a.wdt, a.vec_params, k, 0.f, f);
+#pragma unroll
+      for (int j = 0; j < H; ++j) b[i][j] = f2_of(f[2 * j], f[2 * j + 1]);
+    }
+#pragma unroll
+    for (int j = 0; j < H; ++j) dw[i][j] = db[i][j] = 0;
+  }
+  // first pass: `seg` of a row's `warps` parts, rows r0, r0 + rstep, ...
+  const int lane = tid & 31, warp = tid >> 5, nwarps = blockDim.x >> 5;
+  const int per_warp = 32 / plan.lanes, sub = lane / plan.lanes, t1 = lane - sub * plan.lanes;
+  const int wteams = nwarps / plan.warps, seg = warp % plan.warps;
+  const int r0 = plan.warps > 1 ? warp / plan.warps : warp * per_warp, rstep = wteams * per_warp;
+  for (; row0 < a.M; row0 += tile_step) {
+    const int rows = static_cast<int>(min(static_cast<long long>(plan.rows), a.M - row0));
+    copies_wait(plan.stages);
+    __syncthreads();  // the tile is there for everybody, and nobody reads the tile before any more
+    const uint32_t st = ring + out, dy_at = st + plan.dy_at, x_at = st + plan.x_at, g_at = st + plan.g_at, xs_at = st + plan.xs_at, gs_at = st + plan.gs_at;
+    // an exponent's place: the copied words begin at the last multiple of four before the tile's first
+    const uint32_t skip = SAVED ? static_cast<uint32_t>((row0 * ng) & 3) : 0;
+    out = out + plan.stage_bytes == ring_end ? 0 : out + plan.stage_bytes;
+    start();
+    if (warp < wteams * plan.warps) {
+      for (int base = r0; base < rows; base += rstep) {
+        const int r = base + sub;
+        const bool live = r < rows;
+        const float2 mr = live ? shared_f2(st + plan.st_at + r * 8) : make_float2(0.f, 0.f);
+        const f2 rr = f2_all(mr.y), off = f2_all(-mr.x * mr.y);
+        f2 c1 = 0, c2 = 0;
+#pragma unroll
+        for (int i = 0; i < V1; ++i) {
+          const int k = seg * (32 * V1) + t1 + i * plan.lanes;
+          if (live && k < npack) {
+            f2 xh[H], t[H], wk[H];
+            K::unpack(shared16(dy_at + (r * npack + k) * 16), t);
+            ln_tile_get<DT, SAVED>(x_at, xs_at + skip, r, k, npack, ng, xh);
+            K::plane_get(wplane, npack, k, wk);
+            if constexpr (GATE) {
+              f2 u[H];
+              ln_tile_get<DT, SAVED>(g_at, gs_at + skip, r, k, npack, ng, u);
+#pragma unroll
+              for (int j = 0; j < H; ++j) {
+                const float2 gv = f2_get(u[j]);
+                float s0, s1, rest;
+                ln_sigmoid(gv.x, &s0, &rest);
+                ln_sigmoid(gv.y, &s1, &rest);
+                t[j] = f2_mul(t[j], f2_of(s0, s1));
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < H; ++j) {
+              const f2 u = f2_mul(t[j], wk[j]);
+              c1 = f2_add(c1, u);
+              c2 = f2_fma(u, f2_fma(xh[j], rr, off), c2);
+            }
+          }
+        }
+        float2 cc = make_float2(f2_sum(c1), f2_sum(c2));
+        for (int o = plan.lanes / 2; o > 0; o >>= 1) {
+          cc.x += __shfl_xor_sync(0xffffffffu, cc.x, o);
+          cc.y += __shfl_xor_sync(0xffffffffu, cc.y, o);
+        }
+        if (live && t1 == 0) shared_put(sums + (r * plan.warps + seg) * 8, cc);
+      }
     }
     __syncthreads();
+    if (mine) {
+      char *dx = static_cast<char*>(a.dx) + (row0 + rg) * N * K::ESZ + c * 16, *dg = static_cast<char*>(a.dgate) + (row0 + rg) * N * K::ESZ + c * 16;
+      for (int r = rg; r < rows; r += plan.rg) {
+        const float2 mr = shared_f2(st + plan.st_at + r * 8);
+        float2 cc = shared_f2(sums + r * plan.warps * 8);
+        for (int s = 1; s < plan.warps; ++s) {
+          const float2 more = shared_f2(sums + (r * plan.warps + s) * 8);
+          cc.x += more.x;
+          cc.y += more.y;
+        }
+        const f2 rr = f2_all(mr.y), off = f2_all(-mr.x * mr.y), k1 = f2_all(-cc.x * inv_n * mr.y), k2 = f2_all(-cc.y * inv_n * mr.y);
+#pragma unroll
+        for (int i = 0; i < VP; ++i) {
+          const int k = c + i * plan.ct;
+          if (VP == 1 || k < npack) {
+            f2 xh[H], t[H];
+            K::unpack(shared16(dy_at + (r * npack + k) * 16), t);
+            ln_tile_get<DT, SAVED>(x_at, xs_at + skip, r, k, npack, ng, xh);
+#pragma unroll
+            for (int j = 0; j < H; ++j) xh[j] = f2_fma(xh[j], rr, off);
+            if constexpr (GATE) {
+              f2 u[H];
+              ln_tile_get<DT, SAVED>(g_at, gs_at + skip, r, k, npack, ng, u);
+#pragma unroll
+              for (int j = 0; j < H; ++j) {
+                const float2 gv = f2_get(u[j]);
+                float s0, s1, r0_, r1_;
+                ln_sigmoid(gv.x, &s0, &r0_);
+                ln_sigmoid(gv.y, &s1, &r1_);
+                t[j] = f2_mul(t[j], f2_of(s0, s1));
+                u[j] = f2_mul(f2_mul(t[j], f2_fma(xh[j], w[i][j], b[i][j])), f2_of(r0_, r1_));
+              }
+              if (a.dgate) K::store(dg + i * plan.ct * 16, u);
+            }
+#pragma unroll
+            for (int j = 0; j < H; ++j) {
+              dw[i][j] = f2_fma(t[j], xh[j], dw[i][j]);
+              db[i][j] = f2_add(db[i][j], t[j]);
+              t[j] = f2_fma(f2_mul(t[j], w[i][j]), rr, f2_fma(xh[j], k2, k1));
+            }
+            if (a.dx) K::store(dx + i * plan.ct * 16, t);
+          }
+        }
+        dx += plan.rg * N * K::ESZ;
+        dg += plan.rg * N * K::ESZ;
+      }
+    }
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  if (!a.partial) return;
+  // The CTA's part of dw and db: the sums of rows side by side are added pairwise in a fixed order, through shared memory.
+  float* tree = reinterpret_cast<float*>(ln_shared);
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    float f[VP][P];
+#pragma unroll
+    for (int i = 0; i < VP; ++i) K::floats(which ? db[i] : dw[i], f[i]);
+    for (int left = plan.rg; left > 1;) {
+      const int half = (left + 1) / 2;
+      __syncthreads();
+      if (mine && rg >= half && rg < left)
+#pragma unroll
+        for (int e = 0; e < VP * P; ++e) tree[((rg - half) * VP * P + e) * plan.ct + c] = f[e / P][e % P];
+      __syncthreads();
+      if (rg < left - half)
+#pragma unroll
+        for (int e = 0; e < VP * P; ++e) f[e / P][e % P] += tree[(rg * VP * P + e) * plan.ct + c];
+      left = half;
+    }
+    if (rg == 0) {
+      float* to = a.partial + (static_cast<size_t>(blockIdx.x) * 2 + which) * N;
+#pragma unroll
+      for (int i = 0; i < VP; ++i) {
+        const int k = c + i * plan.ct;
+        if (k < npack)
+#pragma unroll
+          for (int e = 0; e < P; e += 4) reinterpret_cast<float4*>(to + static_cast<size_t>(k) * P)[e / 4] = make_float4(f[i][e], f[i][e + 1], f[i][e + 2], f[i][e + 3]);
+      }
+    }
   }
 }
 

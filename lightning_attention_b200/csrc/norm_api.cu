@@ -4,8 +4,7 @@
 #include <math.h>
 
 #include "../../include/lightning_b200.h"
-#include "launch_count.h"
-#include "layernorm_kernels.cuh"
+#include "layernorm_launch.cuh"
 
 using namespace lab200;
 
@@ -22,31 +21,51 @@ bool size_ok(long long M, int N, long long ld) {
   const long long widest = ld > N ? ld : N;
   return M >= 0 && N >= 1 && N <= (1 << 30) && widest <= (1LL << 58) && (M == 0 || widest <= (1LL << 58) / M);
 }
-unsigned capped(long long want, long long most) { return static_cast<unsigned>(want < 1 ? 1 : want > most ? most : want); }
 
-// Parts that the sums over rows are cut into: one for 32 rows, at most 64.
-int ln_parts(long long M) { return static_cast<int>(M <= 0 ? 0 : M >= 64 * 32 ? 64 : (M + 31) / 32); }
+int sm_count() {
+  int dev = 0, n = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  return n > 0 ? n : 148;
+}
 
-template <int DT>
-int ln_fwd(const LnArgs& a, cudaStream_t st) {
-  ln_fwd_any_kernel<DT><<<capped(a.M, 1 << 20), 256, 0, st>>>(a);
-  return launched();
+bool aligned_params(const LnArgs& a) { return !((reinterpret_cast<uintptr_t>(a.weight) | reinterpret_cast<uintptr_t>(a.bias)) & 15); }
+
+// dw and db from their parts: a CTA per 32 columns, its 32 warps take every 32nd part. No part: zeros.
+__global__ void __launch_bounds__(1024) ln_bwd_join_kernel(const float* __restrict__ partial, int nparts, int N, void* dw, void* db, int wdt) {
+  __shared__ float red[2][32][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (long long c0 = static_cast<long long>(blockIdx.x) * 32; c0 < N; c0 += static_cast<long long>(gridDim.x) * 32) {
+    const int col = static_cast<int>(c0) + lane;
+    const bool on = lane < N - c0;
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll 5
+    for (int p = warp; p < nparts; p += 32) {
+      const float* from = partial + static_cast<size_t>(p) * 2 * N + col;
+      s0 += on ? from[0] : 0.f;
+      s1 += on ? from[N] : 0.f;
+    }
+    red[0][warp][lane] = s0;
+    red[1][warp][lane] = s1;
+    __syncthreads();
+    if (warp < 2) {
+      float v = 0.f;
+#pragma unroll
+      for (int k = 0; k < 32; ++k) v += red[warp][k][lane];
+      if (on) ln_param_out(warp ? db : dw, wdt, col, v);
+    }
+    __syncthreads();
+  }
 }
 
 template <int DT>
-int ln_bwd(LnArgs a, cudaStream_t st) {
-  if (a.M > 0 && (a.dx || a.dgate)) {
-    ln_bwd_any_kernel<DT><<<capped(a.M, 1 << 20), 256, 0, st>>>(a);
-    if (const int rc = launched()) return rc;
+int run_bwd(LnArgs a, cudaStream_t st) {
+  if (a.M > 0) {
+    const LnPlace at{sm_count(), st};
+    if (a.partial) a.nparts = ln_bwd_parts<DT>(a, at);
+    if (ln_bwd<DT>(a, at) != cudaSuccess) return LAB200_ERR_CUDA;
   }
   if (!a.dw && !a.db) return LAB200_OK;
-  const unsigned cols = capped((a.N - 1) / 32 + 1, 1 << 20);
-  a.nparts = ln_parts(a.M);
-  if (a.nparts) {
-    ln_bwd_columns_kernel<DT><<<dim3(cols, a.nparts), 256, 0, st>>>(a);
-    if (const int rc = launched()) return rc;
-  }
-  ln_bwd_join_kernel<<<cols, 256, 0, st>>>(a.partial, a.nparts, a.N, a.dw, a.db, a.wdt);
+  ln_bwd_join_kernel<<<ln_capped((a.N - 1) / 32 + 1, 1 << 20), 1024, 0, st>>>(a.partial, a.nparts, a.N, a.dw, a.db, a.wdt);
   return launched();
 }
 
@@ -68,12 +87,14 @@ int lab200_layernorm_fwd(const void* x, long long ldx, const void* gate, long lo
   a.gcodes = static_cast<int8_t*>(gcodes); a.gscales = static_cast<uint8_t*>(gscales);
   a.M = M; a.N = N; a.eps = eps;
   if (reinterpret_cast<uintptr_t>(stats) & 7) return LAB200_ERR_ALIGN;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == LAB200_F32 ? ln_fwd<SRMS_F32>(a, st) : dtype == LAB200_F16 ? ln_fwd<SRMS_F16>(a, st) : ln_fwd<SRMS_BF16>(a, st);
+  a.vec_params = aligned_params(a);
+  const LnPlace at{sm_count(), static_cast<cudaStream_t>(stream)};
+  const cudaError_t rc = dtype == LAB200_F32 ? ln_fwd<SRMS_F32>(a, at) : dtype == LAB200_F16 ? ln_fwd<SRMS_F16>(a, at) : ln_fwd<SRMS_BF16>(a, at);
+  return rc == cudaSuccess ? LAB200_OK : LAB200_ERR_CUDA;
 }
 
 size_t lab200_layernorm_bwd_workspace_bytes(long long M, int N) {
-  return N < 1 ? 0 : static_cast<size_t>(ln_parts(M)) * 2 * N * sizeof(float);
+  return N < 1 || M < 1 ? 0 : static_cast<size_t>(M < LN_MAX_PARTS ? M : LN_MAX_PARTS) * 2 * N * sizeof(float);
 }
 
 int lab200_layernorm_bwd(const void* x, long long ldx, const void* gate, long long ldg, const void* xcodes, const void* xscales, const void* gcodes,
@@ -96,10 +117,11 @@ int lab200_layernorm_bwd(const void* x, long long ldx, const void* gate, long lo
   a.gcodes = static_cast<int8_t*>(const_cast<void*>(gcodes)); a.gscales = static_cast<uint8_t*>(const_cast<void*>(gscales));
   a.stats = reinterpret_cast<float2*>(const_cast<float*>(stats));
   a.dy = dy; a.lddy = lddy; a.dx = dx; a.dgate = dgate; a.dw = dweight; a.db = dbias;
-  a.partial = static_cast<float*>(workspace);
+  a.partial = dweight || dbias ? static_cast<float*>(workspace) : nullptr;
   a.M = M; a.N = N;
+  a.vec_params = aligned_params(a);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == LAB200_F32 ? ln_bwd<SRMS_F32>(a, st) : dtype == LAB200_F16 ? ln_bwd<SRMS_F16>(a, st) : ln_bwd<SRMS_BF16>(a, st);
+  return dtype == LAB200_F32 ? run_bwd<SRMS_F32>(a, st) : dtype == LAB200_F16 ? run_bwd<SRMS_F16>(a, st) : run_bwd<SRMS_BF16>(a, st);
 }
 
 int lab200_pack8(const void* x, long long ldx, void* codes, void* scales, long long M, int N, int dtype, void* stream) {
@@ -110,7 +132,7 @@ int lab200_pack8(const void* x, long long ldx, void* codes, void* scales, long l
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto* c = static_cast<int8_t*>(codes);
   auto* s = static_cast<uint8_t*>(scales);
-  const unsigned grid = capped((M * ((N - 1) / PK_GROUP + 1) + 7) / 8, 1 << 20);
+  const unsigned grid = ln_capped((M * ((N - 1) / PK_GROUP + 1) + 7) / 8, 1 << 20);
   if (dtype == LAB200_F32) pack8_any_kernel<SRMS_F32><<<grid, 256, 0, st>>>(x, ldx, c, s, M, N);
   else if (dtype == LAB200_F16) pack8_any_kernel<SRMS_F16><<<grid, 256, 0, st>>>(x, ldx, c, s, M, N);
   else pack8_any_kernel<SRMS_BF16><<<grid, 256, 0, st>>>(x, ldx, c, s, M, N);
@@ -125,7 +147,7 @@ int lab200_unpack8(const void* codes, const void* scales, void* y, long long M, 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto* c = static_cast<const int8_t*>(codes);
   auto* s = static_cast<const uint8_t*>(scales);
-  const unsigned grid = capped((M * ((N - 1) / PK_GROUP + 1) + 7) / 8, 1 << 20);
+  const unsigned grid = ln_capped((M * ((N - 1) / PK_GROUP + 1) + 7) / 8, 1 << 20);
   if (dtype == LAB200_F32) unpack8_any_kernel<SRMS_F32><<<grid, 256, 0, st>>>(c, s, y, M, N);
   else if (dtype == LAB200_F16) unpack8_any_kernel<SRMS_F16><<<grid, 256, 0, st>>>(c, s, y, M, N);
   else unpack8_any_kernel<SRMS_BF16><<<grid, 256, 0, st>>>(c, s, y, M, N);

@@ -34,6 +34,52 @@ __device__ __forceinline__ float pk_value(int code, float step) {
   return v;
 }
 
+// The largest magnitude of P values, as bits; a NaN among them wins.
+template <int P>
+__device__ __forceinline__ uint32_t pk_abs_max(const float* f) {
+  float m = fabsf(f[0]);
+#pragma unroll
+  for (int e = 1; e < P; ++e) asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(m), "f"(fabsf(f[e])));
+  return __float_as_uint(m);
+}
+// Its maximum over LANES adjacent lanes, which hold one group.
+template <int LANES>
+__device__ __forceinline__ uint32_t pk_group_max(uint32_t bits) {
+  if constexpr (LANES == 32) return __reduce_max_sync(0xffffffffu, bits);
+#pragma unroll
+  for (int o = 1; o < LANES; o <<= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+  return bits;
+}
+// P codes, four to a word. Adding 1.5 * 2^23 rounds to a whole number, to nearest even, and leaves it in the low byte: exact, as
+// x * inv is. Groups of E = 254 (whose codes may have to be held at 127) and 255 take the checked way.
+template <int P>
+__device__ __forceinline__ void pk_codes(const float* f, uint32_t e, uint32_t* w) {
+  const float inv = pk_inv_step(e);
+  uint32_t c[P];
+  if (e < 254u) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) c[i] = __float_as_uint(fmaf(f[i], inv, 12582912.f));
+  } else {
+#pragma unroll
+    for (int i = 0; i < P; ++i) c[i] = static_cast<uint32_t>(pk_code(f[i], inv));
+  }
+  if constexpr (P == 1) {
+    w[0] = c[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < P; i += 4) w[i / 4] = __byte_perm(__byte_perm(c[i], c[i + 1], 0x0040), __byte_perm(c[i + 2], c[i + 3], 0x0040), 0x5410);
+  }
+}
+// Two adjacent codes of a word as fp32 values: a byte b, moved by 128, in the low byte of 2^23 makes 2^23 + b + 128.
+__device__ __forceinline__ unsigned long long pk_two(uint32_t w, int e) {
+  const uint32_t u = w ^ 0x80808080u;
+  const uint32_t lo = __byte_perm(u, 0x4b000000u, 0x7440 + e), hi = __byte_perm(u, 0x4b000000u, 0x7441 + e);
+  unsigned long long v, r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+  asm("{ .reg .b64 c; mov.b64 c, {%2, %2}; add.rn.f32x2 %0, %1, c; }" : "=l"(r) : "l"(v), "r"(__float_as_uint(-8388736.f)));
+  return r;
+}
+
 // A warp per group, a lane per value: any row length, stride and alignment.
 template <int DT>
 __global__ void __launch_bounds__(256)
