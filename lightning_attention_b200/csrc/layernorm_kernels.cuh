@@ -467,242 +467,309 @@ __global__ void __launch_bounds__(512) ln_fwd_kernel(const LnArgs a, const LnFwd
 }
 
 // ---- backward ----------------------------------------------------------------------------------------------------------------
-// A CTA takes tiles of rows into shared memory and goes over each twice. First warps (or parts of a warp) sum u and u xh over rows,
-// many values of a row to a lane, so that shuffles are few. Behind a barrier every thread has the same VP packs of columns of a number of
-// rows, which are independent of each other: dx and dgate go out, and dw and db are summed in registers.
-struct LnBwdPlan {
-  int ct, rg, rows;    // second pass: threads to a row, rows side by side, rows of a tile
-  int lanes, warps;    // first pass: lanes to a row (a power of two up to 32), warps to a row
-  int stages;
-  uint32_t dy_at, x_at, g_at, st_at, xs_at, gs_at, stage_bytes;  // within a stage
+// A row is a team's of T threads, V packs a thread (E = 16 values), as in the forward pass, and a thread's columns are the same for all
+// rows: it sums dw and db in registers. The copies of a row's dy, x and gate (or their checkpoints) run some rows ahead, into
+// places that are each thread's own.
+constexpr int LN_BWD_THREADS = 512;  // most of a CTA
+constexpr int LN_PITCH = LN_BWD_THREADS * 16;  // bytes from a thread's place for one pack to that for the next
+
+struct LnBwdPlan { int T, stages; };
+
+// What a team reads row by row: a tensor, or (SAVED) its checkpoint.
+template <int DT, int V, bool SAVED>
+struct LnRows {
+  using K = LnPack<DT>;
+  static constexpr int PACK = SAVED ? K::P : 16, PLACE = SAVED ? LN_PITCH / 16 * PACK : LN_PITCH, BYTES = V * PLACE;
+  const char *p, *base;
+  long long step;
+  const uint8_t* e_from;
+  long long e_step;
+  uint32_t at;
+  uint8_t e[SAVED ? V : 1];
+
+  __device__ void init(const void* tensor, long long ld, const int8_t* codes, const uint8_t* scales, int N, long long row, long long rows, int t, uint32_t ring) {
+    base = SAVED ? reinterpret_cast<const char*>(codes) : static_cast<const char*>(tensor);
+    const long long pitch = SAVED ? N : ld * K::ESZ;
+    p = base + row * pitch + t * PACK;
+    step = rows * pitch;
+    at = ring + threadIdx.x * PACK;
+    if constexpr (SAVED) {
+      const int ng = (N - 1) / PK_GROUP + 1;
+      e_from = scales + row * ng + t / K::LANES;
+      e_step = rows * ng;
+    }
+  }
+  // Zeros in the thread's places of a stage: packs behind the row's end are not copied.
+  __device__ void clear(uint32_t stage) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int w = 0; w < PACK / 4; ++w) asm volatile("st.shared.u32 [%0], %1;" ::"r"(stage + at + i * PLACE + 4 * w), "r"(0) : "memory");
+  }
+  // FILL: teams that share a warp, of which one may have no row: its places become zero.
+  template <bool FILL>
+  __device__ void start(uint32_t stage, bool live, int t, int T, int npack) {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (t + i * T < npack) copy_async<PACK>(stage + at + i * PLACE, FILL && !live ? base : p + i * T * PACK, FILL && !live ? 0 : PACK);
+    p += step;
+  }
+  __device__ void start_scales(bool live, int t, int T, int npack) {
+    if constexpr (SAVED) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) e[i] = live && t + i * T < npack ? __ldg(e_from + i * T / K::LANES) : 7;
+      e_from += e_step;
+    }
+  }
+  __device__ void get(uint32_t stage, const uint8_t* ex, f2 (*out)[K::H]) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const uint32_t from = stage + at + i * PLACE;
+      if constexpr (!SAVED) {
+        K::unpack(shared16(from), out[i]);
+      } else {
+        uint32_t w[K::P / 4];
+        if constexpr (K::P == 8) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(from) : "memory");
+        else asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(from) : "memory");
+        const f2 unit = f2_all(pk_step(ex[i]));
+#pragma unroll
+        for (int c = 0; c < K::P; c += 2) out[i][c / 2] = f2_mul(pk_two(w[c / 4], c % 4), unit);
+      }
+    }
+  }
 };
 
-// The exponents of a tile's rows, which lie next to each other in memory, in whole words.
-__device__ __forceinline__ void ln_scales_async(uint32_t to, const uint8_t* from, long long lo, long long hi) {
-  for (long long w = (lo & ~3ll) + 4 * static_cast<long long>(threadIdx.x); w < hi; w += 4 * blockDim.x)
-    copy_async<4>(to + static_cast<uint32_t>(w - (lo & ~3ll)), from + w, hi - w < 4 ? static_cast<int>(hi - w) : 4);
-}
-
-// A pack of x or gate in the backward pass, from its tile in shared memory: the tensor's values, or the checkpoint's.
-template <int DT, bool SAVED>
-__device__ __forceinline__ void ln_tile_get(uint32_t packs, uint32_t exps, int row, int k, int npack, int ng, f2* out) {
-  using K = LnPack<DT>;
-  if constexpr (!SAVED) {
-    K::unpack(shared16(packs + (row * npack + k) * 16), out);
-  } else {
-    uint32_t w[K::P / 4], e;
-    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(e) : "r"(exps + row * ng + k / K::LANES) : "memory");
-    if constexpr (K::P == 8) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(packs + (row * npack + k) * 8) : "memory");
-    else asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(packs + (row * npack + k) * 4) : "memory");
-    const f2 unit = f2_all(pk_step(e));
+// Sums of two values over a team. In a warp the halves exchange what they do not keep, so that both take one shuffle a step. Teams of
+// several warps: `slot` has two halves, used in turn, so that one barrier is enough: who writes a half again has seen everybody
+// arrive at the barrier after the one that guarded its reading. What a team does not fill of `slot` is zero.
+template <int G>
+__device__ __forceinline__ float2 team_sum(float2 v, uint32_t slot, int t, int T, int team) {
+  if constexpr (G < 32) {
 #pragma unroll
-    for (int c = 0; c < K::P; c += 2) out[c / 2] = f2_mul(pk_two(w[c / 4], c % 4), unit);
+    for (int o = G / 2; o > 0; o >>= 1) {
+      v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+      v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    }
+    return v;
+  } else {
+    const bool upper = threadIdx.x & 16;
+    float keep = upper ? v.y : v.x;
+    keep += __shfl_xor_sync(0xffffffffu, upper ? v.x : v.y, 16);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) keep += __shfl_xor_sync(0xffffffffu, keep, o);
+    if constexpr (G == 32) {
+      const float other = __shfl_xor_sync(0xffffffffu, keep, 16);
+      return upper ? make_float2(other, keep) : make_float2(keep, other);
+    } else {
+      if ((t & 15) == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(slot + (t >> 4) * 4), "f"(keep) : "memory");
+      asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(T) : "memory");
+      float4 s = shared_f4(slot);
+      const auto more = [&](int from, int to) {
+#pragma unroll
+        for (int w = from; w < to; ++w) {
+          const float4 u = shared_f4(slot + w * 16);
+          s = make_float4(s.x + u.x, s.y + u.y, s.z + u.z, s.w + u.w);
+        }
+      };
+      if (T > 64) more(1, 2);
+      if (T > 128) more(2, 4);
+      if (T > 256) more(4, 8);
+      if (T > 512) more(8, 10);
+      return make_float2(s.x + s.z, s.y + s.w);
+    }
   }
 }
 
-template <int DT, int VP, bool GATE, bool SAVED>
-__global__ void __launch_bounds__(VP == 1 ? 640 : 512) ln_bwd_kernel(const LnArgs a, const LnBwdPlan plan) {
+template <int DT, int G, bool GATE, bool SAVED>
+__global__ void __launch_bounds__(LN_BWD_THREADS) ln_bwd_kernel(const LnArgs a, const LnBwdPlan plan) {
   using K = LnPack<DT>;
-  constexpr int P = K::P, H = K::H, XP = SAVED ? P : 16;
-  constexpr int V1 = 4;  // packs that a lane sums at a time in the first pass
-  const int N = a.N, npack = N / P, ng = (N - 1) / PK_GROUP + 1, tid = threadIdx.x;
+  constexpr int P = K::P, H = K::H, E = 16, V = E / P;
+  constexpr bool FILL = G < 32;
+  using In = LnRows<DT, V, SAVED>;
+  using Dy = LnRows<DT, V, false>;
+  constexpr uint32_t STAGE = Dy::BYTES + In::BYTES * (GATE ? 2 : 1), SLOTS = G > 32 ? 10 * 2 * 160 : 0;
+  const int T = G <= 32 ? G : plan.T, team = threadIdx.x / T, t = threadIdx.x - team * T, lanes = blockDim.x, teams = lanes / T;
+  const int N = a.N, npack = N / P;
   const float inv_n = 1.f / static_cast<float>(N);
-  const uint32_t wplane = static_cast<uint32_t>(__cvta_generic_to_shared(ln_shared)), sums = wplane + N * 4, ring = sums + ((plan.rows * plan.warps * 8 + 15) & ~15);
-  const uint32_t ring_end = plan.stages * plan.stage_bytes;
-  // this thread's columns and first row in the second pass; `mine` is false for threads that are left over
-  const int rg = tid / plan.ct, c = tid - rg * plan.ct;
-  const bool mine = rg < plan.rg;
-  const long long tile_step = static_cast<long long>(gridDim.x) * plan.rows;
-  long long row0 = static_cast<long long>(blockIdx.x) * plan.rows, ahead = row0;
+  // shared memory: the teams' slots, weight and bias (with a gate, where registers would not do), the ring
+  const uint32_t slots = static_cast<uint32_t>(__cvta_generic_to_shared(ln_shared)), wplane = slots + SLOTS, bplane = wplane + N * 4;
+  const uint32_t ring = GATE ? bplane + N * 4 : wplane, ring_end = plan.stages * STAGE;
+  uint32_t slot = slots + (G > 32 ? team * 320 : 0);
+  if constexpr (G > 32)
+    for (int i = threadIdx.x; i < SLOTS / 4; i += lanes) asm volatile("st.shared.u32 [%0], %1;" ::"r"(slots + 4 * i), "r"(0) : "memory");
+  const long long step = static_cast<long long>(gridDim.x) * teams;
+  const long long row = static_cast<long long>(blockIdx.x) * teams + team;
+  const long long first = FILL ? static_cast<long long>(blockIdx.x) * teams + (threadIdx.x & ~31) / T : row;
+  // rows of this team, and of the team in its warp that has most
+  const int mine = row < a.M ? static_cast<int>((a.M - 1 - row) / step) + 1 : 0, most = first < a.M ? static_cast<int>((a.M - 1 - first) / step) + 1 : 0;
+  In x, g;
+  Dy dy;
+  dy.init(a.dy, a.lddy, nullptr, nullptr, N, row, step, t, ring);
+  x.init(a.x, a.ldx, a.xcodes, a.xscales, N, row, step, t, ring + Dy::BYTES);
+  if constexpr (GATE) g.init(a.gate, a.ldg, a.gcodes, a.gscales, N, row, step, t, ring + Dy::BYTES + In::BYTES);
   uint32_t in = 0, out = 0;
-  const auto start = [&] {
-    if (ahead < a.M) {
-      const int rows = static_cast<int>(min(static_cast<long long>(plan.rows), a.M - ahead));
-      const uint32_t st = ring + in;
-      if (mine) {
-        const char* dy = static_cast<const char*>(a.dy) + (ahead + rg) * a.lddy * K::ESZ;
-        const long long xpitch = SAVED ? N : a.ldx * K::ESZ, gpitch = SAVED ? N : a.ldg * K::ESZ;
-        const char* x = (SAVED ? reinterpret_cast<const char*>(a.xcodes) : static_cast<const char*>(a.x)) + (ahead + rg) * xpitch;
-        const char* g = (SAVED ? reinterpret_cast<const char*>(a.gcodes) : static_cast<const char*>(a.gate)) + (ahead + rg) * gpitch;
-        for (int r = rg; r < rows; r += plan.rg) {
-#pragma unroll
-          for (int i = 0; i < VP; ++i) {
-            const int k = c + i * plan.ct;
-            if (VP == 1 || k < npack) {
-              copy_async<16>(st + plan.dy_at + (r * npack + k) * 16, dy + k * 16);
-              copy_async<XP>(st + plan.x_at + (r * npack + k) * XP, x + k * XP);
-              if constexpr (GATE) copy_async<XP>(st + plan.g_at + (r * npack + k) * XP, g + k * XP);
-            }
-          }
-          dy += plan.rg * a.lddy * K::ESZ;
-          x += plan.rg * xpitch;
-          if constexpr (GATE) g += plan.rg * gpitch;
-        }
-      }
-      for (int r = tid; r < rows; r += blockDim.x) copy_async<8>(st + plan.st_at + r * 8, a.stats + ahead + r);
-      if constexpr (SAVED) {
-        ln_scales_async(st + plan.xs_at, a.xscales, ahead * ng, (ahead + rows) * ng);
-        if constexpr (GATE) ln_scales_async(st + plan.gs_at, a.gscales, ahead * ng, (ahead + rows) * ng);
-      }
+  const auto start = [&](int n) {
+    if (FILL || n < mine) {
+      dy.template start<FILL>(in, n < mine, t, T, npack);
+      x.template start<FILL>(in, n < mine, t, T, npack);
+      if constexpr (GATE) g.template start<FILL>(in, n < mine, t, T, npack);
     }
     copies_commit();
-    ahead += tile_step;
-    in = in + plan.stage_bytes == ring_end ? 0 : in + plan.stage_bytes;
+    in = in + STAGE == ring_end ? 0 : in + STAGE;
   };
-  for (int k = 1; k < plan.stages; ++k) start();
-  f2 w[VP][H], b[GATE ? VP : 1][H], dw[VP][H], db[VP][H];
+  const float2* st_from = a.stats + row;
+  float2 st_next;
+  const auto start_small = [&](int n) {
+    st_next = n < mine ? __ldg(st_from) : make_float2(0.f, 0.f);
+    st_from += step;
+    x.start_scales(n < mine, t, T, npack);
+    if constexpr (GATE) g.start_scales(n < mine, t, T, npack);
+  };
+  for (int k = 0; k < plan.stages; ++k) {
+    dy.clear(k * STAGE);
+    x.clear(k * STAGE);
+    if constexpr (GATE) g.clear(k * STAGE);
+  }
+  for (int k = 1; k < plan.stages; ++k) start(k - 1);
+  start_small(0);
+  f2 w[GATE ? 1 : V][H], dw[V][H], db[V][H];
 #pragma unroll
-  for (int i = 0; i < VP; ++i) {
-    const int k = c + i * plan.ct;
-    float f[P];
-    const bool on = mine && k < npack;
-    K::params(on ? a.weight : nullptr, a.wdt, a.vec_params, k, 1.f, f);
-    if (on && rg == 0) K::plane_put(wplane, npack, k, f);
+  for (int i = 0; i < V; ++i) {
+    const int k = t + i * T;
+    if constexpr (!GATE) {
+      float f[P];
+      K::params(k < npack ? a.weight : nullptr, a.wdt, a.vec_params, k, 1.f, f);
 #pragma unroll
-    for (int j = 0; j < H; ++j) w[i][j] = f2_of(f[2 * j], f[2 * j + 1]);
-    if constexpr (GATE) {
-      K::params(on ? a.bias : nullptr, a.wdt, a.vec_params, k, 0.f, f);
-#pragma unroll
-      for (int j = 0; j < H; ++j) b[i][j] = f2_of(f[2 * j], f[2 * j + 1]);
+      for (int j = 0; j < H; ++j) w[i][j] = f2_of(f[2 * j], f[2 * j + 1]);
     }
 #pragma unroll
     for (int j = 0; j < H; ++j) dw[i][j] = db[i][j] = 0;
   }
-  // first pass: `seg` of a row's `warps` parts, rows r0, r0 + rstep, ...
-  const int lane = tid & 31, warp = tid >> 5, nwarps = blockDim.x >> 5;
-  const int per_warp = 32 / plan.lanes, sub = lane / plan.lanes, t1 = lane - sub * plan.lanes;
-  const int wteams = nwarps / plan.warps, seg = warp % plan.warps;
-  const int r0 = plan.warps > 1 ? warp / plan.warps : warp * per_warp, rstep = wteams * per_warp;
-  for (; row0 < a.M; row0 += tile_step) {
-    const int rows = static_cast<int>(min(static_cast<long long>(plan.rows), a.M - row0));
+  if constexpr (GATE)
+    for (int k = threadIdx.x; k < npack; k += lanes) {
+      float f[P];
+      K::params(a.weight, a.wdt, a.vec_params, k, 1.f, f);
+      K::plane_put(wplane, npack, k, f);
+      K::params(a.bias, a.wdt, a.vec_params, k, 0.f, f);
+      K::plane_put(bplane, npack, k, f);
+    }
+  if constexpr (GATE || G > 32) __syncthreads();
+  char *dx = static_cast<char*>(a.dx) + row * N * K::ESZ + t * 16, *dg = static_cast<char*>(a.dgate) + row * N * K::ESZ + t * 16;
+  const long long out_step = step * N * K::ESZ;
+  for (int n = 0; n < most; ++n, dx += out_step, dg += out_step) {
+    const bool live = !FILL || n < mine;
     copies_wait(plan.stages);
-    __syncthreads();  // the tile is there for everybody, and nobody reads the tile before any more
-    const uint32_t st = ring + out, dy_at = st + plan.dy_at, x_at = st + plan.x_at, g_at = st + plan.g_at, xs_at = st + plan.xs_at, gs_at = st + plan.gs_at;
-    // an exponent's place: the copied words begin at the last multiple of four before the tile's first
-    const uint32_t skip = SAVED ? static_cast<uint32_t>((row0 * ng) & 3) : 0;
-    out = out + plan.stage_bytes == ring_end ? 0 : out + plan.stage_bytes;
-    start();
-    if (warp < wteams * plan.warps) {
-      for (int base = r0; base < rows; base += rstep) {
-        const int r = base + sub;
-        const bool live = r < rows;
-        const float2 mr = live ? shared_f2(st + plan.st_at + r * 8) : make_float2(0.f, 0.f);
-        const f2 rr = f2_all(mr.y), off = f2_all(-mr.x * mr.y);
-        f2 c1 = 0, c2 = 0;
+    const float2 st = st_next;
+    uint8_t ex[SAVED ? V : 1], eg[SAVED && GATE ? V : 1];
+    if constexpr (SAVED) {
 #pragma unroll
-        for (int i = 0; i < V1; ++i) {
-          const int k = seg * (32 * V1) + t1 + i * plan.lanes;
-          if (live && k < npack) {
-            f2 xh[H], t[H], wk[H];
-            K::unpack(shared16(dy_at + (r * npack + k) * 16), t);
-            ln_tile_get<DT, SAVED>(x_at, xs_at + skip, r, k, npack, ng, xh);
-            K::plane_get(wplane, npack, k, wk);
-            if constexpr (GATE) {
-              f2 u[H];
-              ln_tile_get<DT, SAVED>(g_at, gs_at + skip, r, k, npack, ng, u);
-#pragma unroll
-              for (int j = 0; j < H; ++j) {
-                const float2 gv = f2_get(u[j]);
-                float s0, s1, rest;
-                ln_sigmoid(gv.x, &s0, &rest);
-                ln_sigmoid(gv.y, &s1, &rest);
-                t[j] = f2_mul(t[j], f2_of(s0, s1));
-              }
-            }
-#pragma unroll
-            for (int j = 0; j < H; ++j) {
-              const f2 u = f2_mul(t[j], wk[j]);
-              c1 = f2_add(c1, u);
-              c2 = f2_fma(u, f2_fma(xh[j], rr, off), c2);
-            }
-          }
-        }
-        float2 cc = make_float2(f2_sum(c1), f2_sum(c2));
-        for (int o = plan.lanes / 2; o > 0; o >>= 1) {
-          cc.x += __shfl_xor_sync(0xffffffffu, cc.x, o);
-          cc.y += __shfl_xor_sync(0xffffffffu, cc.y, o);
-        }
-        if (live && t1 == 0) shared_put(sums + (r * plan.warps + seg) * 8, cc);
+      for (int i = 0; i < V; ++i) {
+        ex[i] = x.e[i];
+        if constexpr (GATE) eg[i] = g.e[i];
       }
     }
-    __syncthreads();
-    if (mine) {
-      char *dx = static_cast<char*>(a.dx) + (row0 + rg) * N * K::ESZ + c * 16, *dg = static_cast<char*>(a.dgate) + (row0 + rg) * N * K::ESZ + c * 16;
-      for (int r = rg; r < rows; r += plan.rg) {
-        const float2 mr = shared_f2(st + plan.st_at + r * 8);
-        float2 cc = shared_f2(sums + r * plan.warps * 8);
-        for (int s = 1; s < plan.warps; ++s) {
-          const float2 more = shared_f2(sums + (r * plan.warps + s) * 8);
-          cc.x += more.x;
-          cc.y += more.y;
-        }
-        const f2 rr = f2_all(mr.y), off = f2_all(-mr.x * mr.y), k1 = f2_all(-cc.x * inv_n * mr.y), k2 = f2_all(-cc.y * inv_n * mr.y);
+    f2 xh[V][H], s[V][H];
+    dy.get(out, nullptr, s);
+    x.get(out, ex, xh);
+    const f2 rr = f2_all(st.y), off = f2_all(-st.x * st.y);
 #pragma unroll
-        for (int i = 0; i < VP; ++i) {
-          const int k = c + i * plan.ct;
-          if (VP == 1 || k < npack) {
-            f2 xh[H], t[H];
-            K::unpack(shared16(dy_at + (r * npack + k) * 16), t);
-            ln_tile_get<DT, SAVED>(x_at, xs_at + skip, r, k, npack, ng, xh);
+    for (int i = 0; i < V; ++i)
 #pragma unroll
-            for (int j = 0; j < H; ++j) xh[j] = f2_fma(xh[j], rr, off);
-            if constexpr (GATE) {
-              f2 u[H];
-              ln_tile_get<DT, SAVED>(g_at, gs_at + skip, r, k, npack, ng, u);
+      for (int j = 0; j < H; ++j) xh[i][j] = f2_fma(xh[i][j], rr, off);
+    if constexpr (GATE) {
+      f2 u[V][H];
+      g.get(out, eg, u);
 #pragma unroll
-              for (int j = 0; j < H; ++j) {
-                const float2 gv = f2_get(u[j]);
-                float s0, s1, r0_, r1_;
-                ln_sigmoid(gv.x, &s0, &r0_);
-                ln_sigmoid(gv.y, &s1, &r1_);
-                t[j] = f2_mul(t[j], f2_of(s0, s1));
-                u[j] = f2_mul(f2_mul(t[j], f2_fma(xh[j], w[i][j], b[i][j])), f2_of(r0_, r1_));
-              }
-              if (a.dgate) K::store(dg + i * plan.ct * 16, u);
-            }
+      for (int i = 0; i < V; ++i) {
+        const int k = t + i * T;
+        if (k < npack) {
+          f2 wk[H], bk[H];
+          K::plane_get(wplane, npack, k, wk);
+          K::plane_get(bplane, npack, k, bk);
 #pragma unroll
-            for (int j = 0; j < H; ++j) {
-              dw[i][j] = f2_fma(t[j], xh[j], dw[i][j]);
-              db[i][j] = f2_add(db[i][j], t[j]);
-              t[j] = f2_fma(f2_mul(t[j], w[i][j]), rr, f2_fma(xh[j], k2, k1));
-            }
-            if (a.dx) K::store(dx + i * plan.ct * 16, t);
+          for (int j = 0; j < H; ++j) {
+            const float2 gv = f2_get(u[i][j]);
+            float s0, s1, r0, r1;
+            ln_sigmoid(gv.x, &s0, &r0);
+            ln_sigmoid(gv.y, &s1, &r1);
+            s[i][j] = f2_mul(s[i][j], f2_of(s0, s1));
+            u[i][j] = f2_mul(f2_mul(s[i][j], f2_fma(xh[i][j], wk[j], bk[j])), f2_of(r0, r1));
           }
+          if (a.dgate && live) K::store(dg + i * T * 16, u[i]);
         }
-        dx += plan.rg * N * K::ESZ;
-        dg += plan.rg * N * K::ESZ;
       }
     }
+    out = out + STAGE == ring_end ? 0 : out + STAGE;
+    start(n + plan.stages - 1);
+    start_small(n + 1);
+    f2 c1 = 0, c2 = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      f2 wk[H];
+      if constexpr (GATE) {
+#pragma unroll
+        for (int j = 0; j < H; ++j) wk[j] = 0;
+        if (t + i * T < npack) K::plane_get(wplane, npack, t + i * T, wk);
+      }
+#pragma unroll
+      for (int j = 0; j < H; ++j) {
+        const f2 wij = GATE ? wk[j] : w[GATE ? 0 : i][j];
+        db[i][j] = f2_add(db[i][j], s[i][j]);
+        const f2 p = f2_mul(s[i][j], xh[i][j]);
+        dw[i][j] = f2_add(dw[i][j], p);
+        c2 = f2_fma(wij, p, c2);
+        s[i][j] = f2_mul(wij, s[i][j]);
+        c1 = f2_add(c1, s[i][j]);
+      }
+    }
+    const float2 c = team_sum<G>(make_float2(f2_sum(c1), f2_sum(c2)), slot, t, T, team);
+    const f2 k1 = f2_all(-c.x * inv_n * st.y), k2 = f2_all(-c.y * inv_n * st.y);
+    if (a.dx && live) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+#pragma unroll
+        for (int j = 0; j < H; ++j) s[i][j] = f2_fma(s[i][j], rr, f2_fma(xh[i][j], k2, k1));
+        if (t + i * T < npack) K::store(dx + i * T * 16, s[i]);
+      }
+    }
+    if constexpr (G > 32) slot = slots + team * 320 + ((n & 1) ? 0 : 160);
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   if (!a.partial) return;
-  // The CTA's part of dw and db: the sums of rows side by side are added pairwise in a fixed order, through shared memory.
-  float* tree = reinterpret_cast<float*>(ln_shared);
+  // The CTA's part of dw and db: its teams' (for rows within a warp, its warps') sums in their order, through shared memory.
+  constexpr int LW = G < 32 ? G : 32;
+  const int span = G <= 32 ? 32 : T, TT = G <= 32 ? LW : T, units = lanes / span, unit = threadIdx.x / span, tt = threadIdx.x - unit * span;
+  const bool holds = tt < TT;
+  float* sums = reinterpret_cast<float*>(ln_shared);
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
-    float f[VP][P];
+    float acc[E];
 #pragma unroll
-    for (int i = 0; i < VP; ++i) K::floats(which ? db[i] : dw[i], f[i]);
-    for (int left = plan.rg; left > 1;) {
-      const int half = (left + 1) / 2;
+    for (int i = 0; i < V; ++i) K::floats(which ? db[i] : dw[i], acc + i * P);
+#pragma unroll
+    for (int o = LW; o < 32; o <<= 1)
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], o);
+    if (units > 1) {
       __syncthreads();
-      if (mine && rg >= half && rg < left)
+      if (holds && unit > 0)
 #pragma unroll
-        for (int e = 0; e < VP * P; ++e) tree[((rg - half) * VP * P + e) * plan.ct + c] = f[e / P][e % P];
+        for (int e = 0; e < E; ++e) sums[((unit - 1) * E + e) * TT + tt] = acc[e];
       __syncthreads();
-      if (rg < left - half)
+      if (holds && unit == 0)
+        for (int u = 0; u < units - 1; ++u)
 #pragma unroll
-        for (int e = 0; e < VP * P; ++e) f[e / P][e % P] += tree[(rg * VP * P + e) * plan.ct + c];
-      left = half;
+          for (int e = 0; e < E; ++e) acc[e] += sums[(u * E + e) * TT + tt];
     }
-    if (rg == 0) {
+    if (holds && unit == 0) {
       float* to = a.partial + (static_cast<size_t>(blockIdx.x) * 2 + which) * N;
 #pragma unroll
-      for (int i = 0; i < VP; ++i) {
-        const int k = c + i * plan.ct;
+      for (int i = 0; i < V; ++i) {
+        const int k = tt + i * T;
         if (k < npack)
 #pragma unroll
-          for (int e = 0; e < P; e += 4) reinterpret_cast<float4*>(to + static_cast<size_t>(k) * P)[e / 4] = make_float4(f[i][e], f[i][e + 1], f[i][e + 2], f[i][e + 3]);
+          for (int e = 0; e < P; e += 4)
+            reinterpret_cast<float4*>(to + static_cast<size_t>(k) * P)[e / 4] = make_float4(acc[i * P + e], acc[i * P + e + 1], acc[i * P + e + 2], acc[i * P + e + 3]);
       }
     }
   }

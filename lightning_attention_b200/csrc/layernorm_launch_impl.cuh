@@ -74,59 +74,44 @@ cudaError_t ln_fwd(const LnArgs& a, LnPlace at) {
   return ln_fwd_team<DT, 4, 64>(a, at, team(4));
 }
 
-struct LnBwdLaunch { LnBwdPlan plan; int vp, cta; size_t shared; int parts; };
+struct LnBwdLaunch { LnBwdPlan plan; int G, cta; size_t shared; int parts; };
 
-// False: a row has too many packs.
+// False: no kernel that keeps rows in registers takes the call.
 template <int DT>
 bool ln_bwd_plan(const LnArgs& a, LnPlace at, LnBwdLaunch* l) {
   using K = LnPack<DT>;
+  constexpr int E = 16, V = E / K::P;
   const bool gate = a.gate || a.gcodes, saved = a.xcodes;
-  const int npack = a.N / K::P, ng = (a.N - 1) / PK_GROUP + 1;
-  if (!ln_packs(a, K::ESZ) || npack > 512 * 4) return false;
-  l->vp = npack <= 640 ? 1 : npack <= 1024 ? 2 : 4;
-  LnBwdPlan& p = l->plan;
-  p.ct = (npack + l->vp - 1) / l->vp;
-  p.rg = p.ct >= 512 ? 1 : 512 / p.ct;
-  const int kr = 4 / l->vp;
-  int rows = p.rg * kr;
-  if (rows > 512) rows = 512;
-  // few rows: tiles that leave no SM without one
-  const long long fair = (a.M + at.sms - 1) / at.sms;
-  if (rows > fair) rows = static_cast<int>(fair);
-  p.rows = rows;
-  l->cta = (p.rg * p.ct + 31) / 32 * 32;
-  p.lanes = 1;
-  while (p.lanes < 32 && p.lanes * 4 < npack) p.lanes *= 2;
-  p.warps = (npack + 127) / 128;
-  if (p.warps > l->cta / 32) return false;
-  const uint32_t xp = saved ? K::P : 16, tile = static_cast<uint32_t>(rows) * npack;
-  const uint32_t scales = saved ? ((static_cast<uint32_t>(rows) * ng + 3 + 15) & ~15u) : 0;
-  p.dy_at = 0;
-  p.x_at = tile * 16;
-  p.g_at = p.x_at + ((tile * xp + 15) & ~15u);
-  p.st_at = p.g_at + (gate ? ((tile * xp + 15) & ~15u) : 0);
-  p.xs_at = p.st_at + ((static_cast<uint32_t>(rows) * 8 + 15) & ~15u);
-  p.gs_at = p.xs_at + scales;
-  p.stage_bytes = p.gs_at + (gate ? scales : 0);
-  const size_t fixed = static_cast<size_t>(a.N) * 4 + ((rows * p.warps * 8 + 15) & ~15);
-  int stages = static_cast<int>((LN_SHARED - fixed) / p.stage_bytes);
-  if (stages < 2) return false;
-  p.stages = stages > 4 ? 4 : stages;
-  l->shared = fixed + static_cast<size_t>(p.stages) * p.stage_bytes;
-  const size_t tree = static_cast<size_t>(p.rg / 2) * l->vp * K::P * p.ct * 4;
-  if (tree > l->shared) l->shared = tree;
-  const long long tiles = (a.M + rows - 1) / rows;
-  l->parts = static_cast<int>(ln_capped(tiles, at.sms < LN_MAX_PARTS ? at.sms : LN_MAX_PARTS));
-  return true;
+  const int npack = a.N / K::P;
+  if (!ln_packs(a, K::ESZ) || npack > LN_BWD_THREADS * V) return false;
+  const int G = npack <= 8 * V ? 8 : npack <= 16 * V ? 16 : npack <= 32 * V ? 32 : 64;
+  const int T = G <= 32 ? G : (npack + V * 32 - 1) / (V * 32) * 32;
+  l->G = G;
+  // up to 512 threads; one team more where that is a good part of a CTA's
+  int teams = 512 / T;
+  if ((teams + 1) * T <= LN_BWD_THREADS && teams <= 1) ++teams;
+  l->cta = teams * T;
+  const size_t in = static_cast<size_t>(V) * LN_PITCH / 16 * (saved ? K::P : 16), stage = static_cast<size_t>(V) * LN_PITCH + in * (gate ? 2 : 1);
+  const size_t fixed = (G > 32 ? 10 * 2 * 160 : 0) + (gate ? static_cast<size_t>(a.N) * 8 : 0);
+  const int units = l->cta / (G <= 32 ? 32 : T);
+  const size_t sums = static_cast<size_t>(units - 1) * E * T * 4;
+  const int stages = static_cast<int>((LN_SHARED - fixed) / stage);
+  if (fixed > LN_SHARED || stages < 2) return false;
+  l->plan = {T, stages > 4 ? 4 : stages};
+  l->shared = fixed + l->plan.stages * stage;
+  if (sums > l->shared) l->shared = sums;
+  const long long ctas = (a.M + teams - 1) / teams;
+  l->parts = static_cast<int>(ln_capped(ctas, at.sms < LN_MAX_PARTS ? at.sms : LN_MAX_PARTS));
+  return (a.M + teams - 1) / teams / l->parts < (1 << 30);
 }
 
-template <int DT, int VP>
-cudaError_t ln_bwd_packs(const LnArgs& a, LnPlace at, const LnBwdLaunch& l) {
+template <int DT, int G>
+cudaError_t ln_bwd_team(const LnArgs& a, LnPlace at, const LnBwdLaunch& l) {
   const bool gate = a.gate || a.gcodes, saved = a.xcodes;
-  if (gate) return saved ? ln_launch(ln_bwd_kernel<DT, VP, true, true>, l.parts, l.cta, l.shared, at.st, a, l.plan)
-                         : ln_launch(ln_bwd_kernel<DT, VP, true, false>, l.parts, l.cta, l.shared, at.st, a, l.plan);
-  return saved ? ln_launch(ln_bwd_kernel<DT, VP, false, true>, l.parts, l.cta, l.shared, at.st, a, l.plan)
-               : ln_launch(ln_bwd_kernel<DT, VP, false, false>, l.parts, l.cta, l.shared, at.st, a, l.plan);
+  if (gate) return saved ? ln_launch(ln_bwd_kernel<DT, G, true, true>, l.parts, l.cta, l.shared, at.st, a, l.plan)
+                         : ln_launch(ln_bwd_kernel<DT, G, true, false>, l.parts, l.cta, l.shared, at.st, a, l.plan);
+  return saved ? ln_launch(ln_bwd_kernel<DT, G, false, true>, l.parts, l.cta, l.shared, at.st, a, l.plan)
+               : ln_launch(ln_bwd_kernel<DT, G, false, false>, l.parts, l.cta, l.shared, at.st, a, l.plan);
 }
 
 template <int DT>
@@ -138,7 +123,8 @@ int ln_bwd_parts(const LnArgs& a, LnPlace at) {
 template <int DT>
 cudaError_t ln_bwd(LnArgs a, LnPlace at) {
   LnBwdLaunch l;
-  if (ln_bwd_plan<DT>(a, at, &l)) return l.vp == 1 ? ln_bwd_packs<DT, 1>(a, at, l) : l.vp == 2 ? ln_bwd_packs<DT, 2>(a, at, l) : ln_bwd_packs<DT, 4>(a, at, l);
+  if (ln_bwd_plan<DT>(a, at, &l))
+    return l.G == 8 ? ln_bwd_team<DT, 8>(a, at, l) : l.G == 16 ? ln_bwd_team<DT, 16>(a, at, l) : l.G == 32 ? ln_bwd_team<DT, 32>(a, at, l) : ln_bwd_team<DT, 64>(a, at, l);
   if (a.dx || a.dgate) {
     ln_bwd_any_kernel<DT><<<ln_capped(a.M, 1 << 20), 256, 0, at.st>>>(a);
     count_launch();
