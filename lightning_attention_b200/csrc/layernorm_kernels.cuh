@@ -64,7 +64,7 @@ __device__ __forceinline__ float ln_rstd(float d1, float d2, float eps) {
 // One value of x or gate in the backward pass, from the tensor or from its checkpoint.
 template <int DT>
 __device__ __forceinline__ float ln_saved(const void* p, long long ld, const int8_t* codes, const uint8_t* scales, long long row, int col, int N) {
-  if (codes) return pk_value<SRMS_F32>(codes[row * N + col], pk_step(scales[row * ((N - 1) / PK_GROUP + 1) + col / PK_GROUP]));
+  if (codes) return static_cast<float>(codes[row * N + col]) * (pk_step(scales[row * ((N - 1) / PK_GROUP + 1) + col / PK_GROUP]));
   return SrmsElem<DT>::ld(static_cast<const typename SrmsElem<DT>::T*>(p) + row * ld + col);
 }
 

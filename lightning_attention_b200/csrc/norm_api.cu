@@ -28,6 +28,20 @@ int sm_count() {
   return n > 0 ? n : 148;
 }
 
+// How a call's rows are given out to warps: by packs of P values, or (P 0) by groups. Contiguous rows of whole groups are one row.
+constexpr int PK_U = 4;
+PkRows pk_rows(long long M, long long N, int P, bool contiguous) {
+  if (P && contiguous && N % PK_GROUP == 0) N *= M, M = 1;
+  PkRows r;
+  r.M = M;
+  r.ngroups = (N - 1) / PK_GROUP + 1;
+  r.npack = P ? N / P : N;
+  const long long units = P ? r.ngroups * (PK_GROUP / P) : r.ngroups, per = P ? 32 * PK_U : PK_U, per_row = (units + per - 1) / per;
+  r.items = M * per_row;
+  r.per_row = M == 1 ? 0 : static_cast<int>(per_row);
+  return r;
+}
+
 bool aligned_params(const LnArgs& a) { return !((reinterpret_cast<uintptr_t>(a.weight) | reinterpret_cast<uintptr_t>(a.bias)) & 15); }
 
 // dw and db from their parts: a CTA per 32 columns, its 32 warps take every 32nd part. No part: zeros.
@@ -129,13 +143,21 @@ int lab200_pack8(const void* x, long long ldx, void* codes, void* scales, long l
   if (!dtype_known(dtype)) return LAB200_ERR_DTYPE;
   if (M == 0) return LAB200_OK;
   if (!x || !codes || !scales) return LAB200_ERR_SHAPE;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (M == 1) ldx = N;
+  const int esz = dtype == LAB200_F32 ? 4 : 2;
   auto* c = static_cast<int8_t*>(codes);
   auto* s = static_cast<uint8_t*>(scales);
-  const unsigned grid = ln_capped((M * ((N - 1) / PK_GROUP + 1) + 7) / 8, 1 << 20);
-  if (dtype == LAB200_F32) pack8_any_kernel<SRMS_F32><<<grid, 256, 0, st>>>(x, ldx, c, s, M, N);
-  else if (dtype == LAB200_F16) pack8_any_kernel<SRMS_F16><<<grid, 256, 0, st>>>(x, ldx, c, s, M, N);
-  else pack8_any_kernel<SRMS_BF16><<<grid, 256, 0, st>>>(x, ldx, c, s, M, N);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool packs = !((reinterpret_cast<uintptr_t>(x) | static_cast<uintptr_t>(ldx) * esz | static_cast<uintptr_t>(N) * esz) & 15) &&
+                     !(reinterpret_cast<uintptr_t>(codes) % (16 / esz));
+  const PkRows r = pk_rows(M, N, packs ? 16 / esz : 0, ldx == N);
+  const unsigned grid = ln_capped((r.items + 7) / 8, 16LL * sm_count());
+#define LAB200_PACK(DT) \
+  packs ? pack8_kernel<DT, PK_U><<<grid, 256, 0, st>>>(x, ldx, c, s, r) : pack8_any_kernel<DT, PK_U><<<grid, 256, 0, st>>>(x, ldx, c, s, N, r)
+  if (dtype == LAB200_F32) LAB200_PACK(SRMS_F32);
+  else if (dtype == LAB200_F16) LAB200_PACK(SRMS_F16);
+  else LAB200_PACK(SRMS_BF16);
+#undef LAB200_PACK
   return launched();
 }
 
@@ -144,13 +166,19 @@ int lab200_unpack8(const void* codes, const void* scales, void* y, long long M, 
   if (!dtype_known(dtype)) return LAB200_ERR_DTYPE;
   if (M == 0) return LAB200_OK;
   if (!y || !codes || !scales) return LAB200_ERR_SHAPE;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int esz = dtype == LAB200_F32 ? 4 : 2;
   auto* c = static_cast<const int8_t*>(codes);
   auto* s = static_cast<const uint8_t*>(scales);
-  const unsigned grid = ln_capped((M * ((N - 1) / PK_GROUP + 1) + 7) / 8, 1 << 20);
-  if (dtype == LAB200_F32) unpack8_any_kernel<SRMS_F32><<<grid, 256, 0, st>>>(c, s, y, M, N);
-  else if (dtype == LAB200_F16) unpack8_any_kernel<SRMS_F16><<<grid, 256, 0, st>>>(c, s, y, M, N);
-  else unpack8_any_kernel<SRMS_BF16><<<grid, 256, 0, st>>>(c, s, y, M, N);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool packs = !((reinterpret_cast<uintptr_t>(y) | static_cast<uintptr_t>(N) * esz) & 15) && !(reinterpret_cast<uintptr_t>(codes) % (16 / esz));
+  const PkRows r = pk_rows(M, N, packs ? 16 / esz : 0, true);
+  const unsigned grid = ln_capped((r.items + 7) / 8, 16LL * sm_count());
+#define LAB200_UNPACK(DT) \
+  packs ? unpack8_kernel<DT, PK_U><<<grid, 256, 0, st>>>(c, s, y, r) : unpack8_any_kernel<DT, PK_U><<<grid, 256, 0, st>>>(c, s, y, N, r)
+  if (dtype == LAB200_F32) LAB200_UNPACK(SRMS_F32);
+  else if (dtype == LAB200_F16) LAB200_UNPACK(SRMS_F16);
+  else LAB200_UNPACK(SRMS_BF16);
+#undef LAB200_UNPACK
   return launched();
 }
 

@@ -26,11 +26,10 @@ __device__ __forceinline__ float pk_inv_step(uint32_t e) { return __uint_as_floa
 // The code of one value; a group of E = 255 gets zeros (inv = 0 makes 0 or NaN of its values, and NaN converts to 0).
 __device__ __forceinline__ int pk_code(float x, float inv) { return min(max(__float2int_rn(x * inv), -127), 127); }
 
-// A checkpoint's value in a 16-bit type: exact, but that a group's largest fp16 value may round up past 65504.
+// A checkpoint's value before it becomes fp16: what rounded up past the type's largest value is held there. A NaN stays one.
 template <int DT>
-__device__ __forceinline__ float pk_value(int code, float step) {
-  float v = static_cast<float>(code) * step;
-  if constexpr (DT == SRMS_F16) v = v > 65504.f ? 65504.f : v < -65504.f ? -65504.f : v;  // comparisons keep a NaN
+__device__ __forceinline__ float pk_bound(float v) {
+  if constexpr (DT == SRMS_F16) v = v > 65504.f ? 65504.f : v < -65504.f ? -65504.f : v;
   return v;
 }
 
@@ -80,36 +79,153 @@ __device__ __forceinline__ unsigned long long pk_two(uint32_t w, int e) {
   return r;
 }
 
-// A warp per group, a lane per value: any row length, stride and alignment.
-template <int DT>
-__global__ void __launch_bounds__(256)
-pack8_any_kernel(const void* __restrict__ x_, long long ldx, int8_t* __restrict__ codes, uint8_t* __restrict__ scales, long long M, int N) {
-  using E = SrmsElem<DT>;
-  const auto* x = static_cast<const typename E::T*>(x_);
-  const int ng = (N - 1) / PK_GROUP + 1, lane = threadIdx.x & 31;
-  const long long total = M * ng, step = static_cast<long long>(gridDim.x) * 8;
-  for (long long g = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5); g < total; g += step) {
-    const long long row = g / ng;
-    const int col = static_cast<int>(g - row * ng) * PK_GROUP + lane;
-    const bool on = lane < N - (col - lane);
-    const float v = on ? E::ld(x + row * ldx + col) : 0.f;
-    const uint32_t e = pk_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(v))));
-    if (on) codes[row * N + col] = static_cast<int8_t>(pk_code(v, pk_inv_step(e)));
-    if (lane == 0) scales[g] = static_cast<uint8_t>(e);
+// ---- pack and unpack on their own: streaming kernels, bound by memory (3 1/32 bytes for each 16-bit value) -----------------------
+// Where packs of 16 bytes divide the rows: a warp takes 32 * U adjacent packs of a row at a time, a lane every 32nd, so that LANES
+// adjacent lanes hold a group and U accesses are under way. `npack` packs to a row; contiguous rows of whole groups come as one row.
+struct PkRows { long long M, npack, ngroups, items; int per_row; };
+
+__device__ __forceinline__ void pk_item(const PkRows& r, long long item, long long* row, long long* k) {
+  if (r.M == 1) {
+    *row = 0;
+    *k = item;
+  } else if (item < (1ll << 31)) {  // a division in 32 bits
+    *row = static_cast<uint32_t>(item) / static_cast<uint32_t>(r.per_row);
+    *k = item - *row * r.per_row;
+  } else {
+    *row = item / r.per_row;
+    *k = item - *row * r.per_row;
   }
 }
 
-template <int DT>
+template <int DT, int U>
 __global__ void __launch_bounds__(256)
-unpack8_any_kernel(const int8_t* __restrict__ codes, const uint8_t* __restrict__ scales, void* __restrict__ y_, long long M, int N) {
+pack8_kernel(const void* __restrict__ x_, long long ldx, int8_t* __restrict__ codes, uint8_t* __restrict__ scales, const PkRows r) {
+  constexpr int P = SrmsVec<DT>::EPV, LANES = PK_GROUP / P, ESZ = 16 / P;
+  const int lane = threadIdx.x & 31;
+  const long long step = static_cast<long long>(gridDim.x) * 8;
+  for (long long item = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5); item < r.items; item += step) {
+    long long row, k0;
+    pk_item(r, item, &row, &k0);
+    k0 = k0 * (32 * U) + lane;
+    const auto* x = reinterpret_cast<const SrmsPack<1>*>(static_cast<const char*>(x_) + row * ldx * ESZ);
+    SrmsPack<1> v[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      v[i].q[0] = make_uint4(0, 0, 0, 0);
+      if (k0 + 32 * i < r.npack) v[i] = ld_stream<1>(x + k0 + 32 * i);
+    }
+    auto* to = reinterpret_cast<uint32_t*>(codes + row * r.npack * P);
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const long long k = k0 + 32 * i;
+      float f[P];
+      SrmsVec<DT>::unpack(v[i].q[0], f);
+      const uint32_t e = pk_exponent(pk_group_max<LANES>(pk_abs_max<P>(f)));
+      uint32_t w[P / 4];
+      pk_codes<P>(f, e, w);
+      if (k < r.npack) {
+        if constexpr (P == 8) reinterpret_cast<uint2*>(to)[k] = make_uint2(w[0], w[1]);
+        else to[k] = w[0];
+        if (k % LANES == 0) scales[row * r.ngroups + k / LANES] = static_cast<uint8_t>(e);
+      }
+    }
+  }
+}
+
+template <int DT, int U>
+__global__ void __launch_bounds__(256)
+unpack8_kernel(const int8_t* __restrict__ codes, const uint8_t* __restrict__ scales, void* __restrict__ y_, const PkRows r) {
+  constexpr int P = SrmsVec<DT>::EPV, LANES = PK_GROUP / P;
+  const int lane = threadIdx.x & 31;
+  const long long step = static_cast<long long>(gridDim.x) * 8;
+  for (long long item = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5); item < r.items; item += step) {
+    long long row, k0;
+    pk_item(r, item, &row, &k0);
+    k0 = k0 * (32 * U) + lane;
+    const auto* from = reinterpret_cast<const uint32_t*>(codes + row * r.npack * P);
+    auto* y = reinterpret_cast<SrmsPack<1>*>(y_) + row * r.npack;
+    uint32_t w[U][P / 4], e[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const long long k = k0 + 32 * i;
+      if (k < r.npack) {
+        if constexpr (P == 8) {
+          const uint2 v = __ldcs(reinterpret_cast<const uint2*>(from) + k);
+          w[i][0] = v.x; w[i][P / 4 - 1] = v.y;
+        } else {
+          w[i][0] = __ldcs(from + k);
+        }
+        e[i] = __ldg(scales + row * r.ngroups + k / LANES);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const long long k = k0 + 32 * i;
+      if (k < r.npack) {
+        const float unit = pk_step(e[i]);
+        float f[P];
+#pragma unroll
+        for (int c = 0; c < P; c += 2) {
+          const unsigned long long two = pk_two(w[i][c / 4], c % 4);
+          float lo, hi;
+          asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(two));
+          f[c] = pk_bound<DT>(lo * unit);
+          f[c + 1] = pk_bound<DT>(hi * unit);
+        }
+        SrmsPack<1> o;
+        o.q[0] = SrmsVec<DT>::pack(f);
+        st_stream<1>(y + k, o);
+      }
+    }
+  }
+}
+
+// Any row length, stride and alignment: a warp takes U adjacent groups of a row at a time, a lane a value of each.
+template <int DT, int U>
+__global__ void __launch_bounds__(256)
+pack8_any_kernel(const void* __restrict__ x_, long long ldx, int8_t* __restrict__ codes, uint8_t* __restrict__ scales, int N, const PkRows r) {
   using E = SrmsElem<DT>;
-  auto* y = static_cast<typename E::T*>(y_);
-  const int ng = (N - 1) / PK_GROUP + 1, lane = threadIdx.x & 31;
-  const long long total = M * ng, step = static_cast<long long>(gridDim.x) * 8;
-  for (long long g = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5); g < total; g += step) {
-    const long long row = g / ng;
-    const int col = static_cast<int>(g - row * ng) * PK_GROUP + lane;
-    if (lane < N - (col - lane)) E::st(y + row * N + col, pk_value<DT>(codes[row * N + col], pk_step(scales[g])));
+  const int lane = threadIdx.x & 31;
+  const long long step = static_cast<long long>(gridDim.x) * 8;
+  for (long long item = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5); item < r.items; item += step) {
+    long long row, k0;
+    pk_item(r, item, &row, &k0);
+    const auto* x = static_cast<const typename E::T*>(x_) + row * ldx;
+    const int g0 = static_cast<int>(k0) * U, c0 = g0 * PK_GROUP + lane;
+    float v[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) v[i] = c0 + i * PK_GROUP < N ? E::ld(x + c0 + i * PK_GROUP) : 0.f;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const uint32_t e = pk_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(v[i]))));
+      if (c0 + i * PK_GROUP < N) codes[row * N + c0 + i * PK_GROUP] = static_cast<int8_t>(pk_code(v[i], pk_inv_step(e)));
+      if (lane == 0 && g0 + i < r.ngroups) scales[row * r.ngroups + g0 + i] = static_cast<uint8_t>(e);
+    }
+  }
+}
+
+template <int DT, int U>
+__global__ void __launch_bounds__(256)
+unpack8_any_kernel(const int8_t* __restrict__ codes, const uint8_t* __restrict__ scales, void* __restrict__ y_, int N, const PkRows r) {
+  using E = SrmsElem<DT>;
+  const int lane = threadIdx.x & 31;
+  const long long step = static_cast<long long>(gridDim.x) * 8;
+  for (long long item = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5); item < r.items; item += step) {
+    long long row, k0;
+    pk_item(r, item, &row, &k0);
+    auto* y = static_cast<typename E::T*>(y_) + row * N;
+    const int g0 = static_cast<int>(k0) * U, c0 = g0 * PK_GROUP + lane;
+    int v[U];
+    uint32_t e[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (c0 + i * PK_GROUP < N) {
+        v[i] = codes[row * N + c0 + i * PK_GROUP];
+        e[i] = __ldg(scales + row * r.ngroups + g0 + i);
+      }
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (c0 + i * PK_GROUP < N) E::st(y + c0 + i * PK_GROUP, pk_bound<DT>(static_cast<float>(v[i]) * pk_step(e[i])));
   }
 }
 
