@@ -94,7 +94,8 @@ def lib():
 _host = None
 _HOST_ENTRIES = ("lab200_error_string", "lab200_last_status", "lab200_la_plan_chunks", "lab200_la_workspace_bytes", "lab200_la_generic",
                  "lab200_la_decode_step", "lab200_la2_fwd", "lab200_la2_bwd", "lab200_la2_bwd_workspace_bytes", "lab200_la2_bwd_kept", "lab200_srmsnorm_fwd", "lab200_srmsnorm_bwd",
-                 "lab200_srmsnorm_gate_fwd", "lab200_srmsnorm_gate_bwd")
+                 "lab200_srmsnorm_gate_fwd", "lab200_srmsnorm_gate_bwd", "lab200_layernorm_fwd", "lab200_layernorm_bwd",
+                 "lab200_layernorm_bwd_workspace_bytes", "lab200_pack8", "lab200_unpack8")
 
 
 HOST_PATH = os.path.join(_HERE, "_host_ops.so")

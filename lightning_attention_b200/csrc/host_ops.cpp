@@ -35,6 +35,11 @@ struct Api {
   decltype(&lab200_srmsnorm_bwd) srms_bwd;
   decltype(&lab200_srmsnorm_gate_fwd) gate_fwd;
   decltype(&lab200_srmsnorm_gate_bwd) gate_bwd;
+  decltype(&lab200_layernorm_fwd) ln_fwd;
+  decltype(&lab200_layernorm_bwd) ln_bwd;
+  decltype(&lab200_layernorm_bwd_workspace_bytes) ln_bwd_workspace_bytes;
+  decltype(&lab200_pack8) pack8;
+  decltype(&lab200_unpack8) unpack8;
 };
 Api g_api{};
 
@@ -61,6 +66,11 @@ void bind(const std::unordered_map<std::string, uintptr_t>& t) {
   set_entry(t, "lab200_srmsnorm_bwd", a.srms_bwd);
   set_entry(t, "lab200_srmsnorm_gate_fwd", a.gate_fwd);
   set_entry(t, "lab200_srmsnorm_gate_bwd", a.gate_bwd);
+  set_entry(t, "lab200_layernorm_fwd", a.ln_fwd);
+  set_entry(t, "lab200_layernorm_bwd", a.ln_bwd);
+  set_entry(t, "lab200_layernorm_bwd_workspace_bytes", a.ln_bwd_workspace_bytes);
+  set_entry(t, "lab200_pack8", a.pack8);
+  set_entry(t, "lab200_unpack8", a.unpack8);
   g_api = a;
 }
 
@@ -335,6 +345,165 @@ std::optional<Tensor> norm_gate(const Tensor& x, const Tensor& gate, double eps)
   return NormGate::apply(x, gate, eps);
 }
 
+// ---- layer norm, with or without a gate ------------------------------------------------------------------------------------
+bool row_type(const Tensor& x) {
+  const auto t = x.scalar_type();
+  return t == at::kFloat || t == at::kHalf || t == at::kBFloat16;
+}
+// Rows that are read in place: a contiguous tensor, or a matrix of any row stride.
+bool rows_in_place(const Tensor& x) {
+  return x.dim() >= 1 && x.numel() > 0 && x.size(-1) <= (1 << 30) &&
+         (x.is_contiguous() || (x.dim() == 2 && x.stride(1) == 1 && (x.size(0) == 1 || x.stride(0) >= x.size(1))));
+}
+struct Rows {
+  int64_t N, M, ld;
+  explicit Rows(const Tensor& x) : N(x.size(-1)), M(x.numel() / N), ld(!x.is_contiguous() && M > 1 ? x.stride(0) : N) {}
+};
+Tensor to_rows(const Tensor& x) { return rows_in_place(x) ? x : x.contiguous(); }
+int64_t groups(int64_t N) { return (N + 31) / 32; }
+
+bool plain_param(const std::optional<Tensor>& p, const Tensor& x) {
+  return !p || (plain(*p) && p->dim() == 1 && p->size(0) == x.size(-1) && p->is_contiguous() && p->device() == x.device() &&
+                (p->scalar_type() == x.scalar_type() || p->scalar_type() == at::kFloat));
+}
+const void* ptr_or_null(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+void* out_or_null(Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
+Tensor bytes(int64_t rows, int64_t cols, const Tensor& like, at::ScalarType type) {
+  return at::empty({rows, cols}, like.options().dtype(type).requires_grad(false));
+}
+
+// What the backward pass works from; `xs` and `gs` only with 8-bit checkpoints, which then stand in place of x and gate.
+struct LnSaved { Tensor stats, x, xs, g, gs; };
+
+Tensor layer_norm_forward(const Tensor& x, const Tensor& gate, const Tensor& weight, const Tensor& bias, double eps, bool save8, LnSaved* saved) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Rows r(x), rg(gate.defined() ? gate : x);
+  Tensor y = at::empty(x.sizes(), x.options().requires_grad(false));
+  Tensor stats, xc, xs, gc, gs;
+  if (saved) {
+    stats = bytes(r.M, 2, x, at::kFloat);
+    if (save8) {
+      xc = bytes(r.M, r.N, x, at::kChar); xs = bytes(r.M, groups(r.N), x, at::kByte);
+      if (gate.defined()) { gc = bytes(r.M, r.N, x, at::kChar); gs = bytes(r.M, groups(r.N), x, at::kByte); }
+    }
+  }
+  const int wdt = weight.defined() ? dtype_code(weight) : bias.defined() ? dtype_code(bias) : LAB200_F32;
+  check(g_api.ln_fwd(x.const_data_ptr(), r.ld, ptr_or_null(gate), rg.ld, ptr_or_null(weight), ptr_or_null(bias), wdt, y.mutable_data_ptr(),
+                     static_cast<float*>(out_or_null(stats)), out_or_null(xc), out_or_null(xs), out_or_null(gc), out_or_null(gs), r.M,
+                     static_cast<int>(r.N), static_cast<float>(eps), dtype_code(x), stream_of(x)), "lab200_layernorm_fwd");
+  if (saved) *saved = {stats, save8 ? xc : x, xs, save8 ? gc : gate, gs};
+  return y;
+}
+
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& gate, const std::optional<Tensor>& weight,
+                        const std::optional<Tensor>& bias, double eps, bool save8) {
+    const Tensor g = gate.value_or(Tensor()), w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+    LnSaved s;
+    Tensor y = layer_norm_forward(x, g, w, b, eps, save8, &s);
+    ctx->save_for_backward({s.x, s.xs, s.g, s.gs, s.stats, w, g.defined() ? b : Tensor()});
+    ctx->saved_data["rows"] = x.numel() / x.size(-1);
+    ctx->saved_data["width"] = x.size(-1);
+    ctx->saved_data["type"] = static_cast<int64_t>(x.scalar_type());
+    ctx->saved_data["params"] = static_cast<int64_t>(w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : at::kFloat);
+    // which tensors there were, in the order of the node's inputs
+    ctx->saved_data["given"] = (g.defined() ? 1 : 0) | (w.defined() ? 2 : 0) | (b.defined() ? 4 : 0) | (save8 ? 8 : 0);
+    return y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "layer norm can be differentiated once only: its backward pass does not run with create_graph=True");
+    const variable_list saved = ctx->get_saved_variables();
+    const int64_t M = ctx->saved_data["rows"].toInt(), N = ctx->saved_data["width"].toInt(), given = ctx->saved_data["given"].toInt();
+    const auto type = static_cast<at::ScalarType>(ctx->saved_data["type"].toInt()), ptype = static_cast<at::ScalarType>(ctx->saved_data["params"].toInt());
+    const bool gated = given & 1, save8 = given & 8;
+    Tensor dy = grads[0];
+    TORCH_CHECK(dy.numel() == M * N && dy.size(-1) == N, "gradient and input sizes differ");
+    const auto device = dy.device();
+    const c10::cuda::CUDAGuard guard(device);
+    const auto is = [&](const Tensor& t, at::ScalarType want, int64_t rows, int64_t cols) {
+      return t.defined() && t.dim() >= 1 && t.scalar_type() == want && t.device() == device && t.numel() == rows * cols && t.size(-1) == cols;
+    };
+    bool fits = is(saved[4], at::kFloat, M, 2);
+    for (int i : {0, 2}) {
+      if (i == 2 && !gated) break;
+      fits = fits && (save8 ? is(saved[i], at::kChar, M, N) && is(saved[i + 1], at::kByte, M, groups(N)) : is(saved[i], type, M, N));
+    }
+    for (int i : {5, 6}) fits = fits && (!saved[i].defined() || is(saved[i], ptype, 1, N));
+    TORCH_CHECK(fits, "layer norm backward: saved-tensor hooks returned another shape, dtype or device");
+    const Tensor stats = saved[4].contiguous(), w = saved[5].defined() ? saved[5].contiguous() : saved[5], b = saved[6].defined() ? saved[6].contiguous() : saved[6];
+    Tensor x = saved[0], xs = saved[1], g = saved[2], gs = saved[3];
+    if (save8) {
+      x = x.contiguous(); xs = xs.contiguous();
+      if (gated) { g = g.contiguous(); gs = gs.contiguous(); }
+    } else {
+      x = to_rows(x);
+      if (gated) g = to_rows(g);
+    }
+    dy = to_rows(dy.to(type));
+    // the node's inputs are x and those of gate, weight and bias that there were
+    size_t edge = 0;
+    const bool need_x = ctx->needs_input_grad(edge++), need_g = gated && ctx->needs_input_grad(edge++);
+    const bool need_w = (given & 2) && ctx->needs_input_grad(edge++), need_b = (given & 4) && ctx->needs_input_grad(edge++);
+    const auto opt = dy.options().requires_grad(false);
+    Tensor dx, dg, dw, db;
+    if (need_x) dx = at::empty(grads[0].sizes(), opt);
+    if (need_g) dg = at::empty(grads[0].sizes(), opt);
+    if (need_w) dw = at::empty({N}, opt.dtype(ptype));
+    if (need_b) db = at::empty({N}, opt.dtype(ptype));
+    const size_t nbytes = need_w || need_b ? g_api.ln_bwd_workspace_bytes(M, static_cast<int>(N)) : 0;
+    Tensor ws = nbytes ? workspace(nbytes, dy) : Tensor();
+    const Rows rx(x), rg(gated ? g : x), rdy(dy);
+    const int wdt = ptype == at::kFloat ? LAB200_F32 : ptype == at::kHalf ? LAB200_F16 : LAB200_BF16;
+    const void *xp = x.const_data_ptr(), *gp = gated ? g.const_data_ptr() : nullptr;
+    check(g_api.ln_bwd(save8 ? nullptr : xp, rx.ld, save8 ? nullptr : gp, rg.ld, save8 ? xp : nullptr, ptr_or_null(xs), save8 ? gp : nullptr,
+                       ptr_or_null(gs), float_ptr(stats), dy.const_data_ptr(), rdy.ld, ptr_or_null(w), ptr_or_null(b), wdt, out_or_null(dx),
+                       out_or_null(dg), out_or_null(dw), out_or_null(db), out_or_null(ws), nbytes, M, static_cast<int>(N), dtype_code(dy),
+                       stream_of(dy)), "lab200_layernorm_bwd");
+    return {dx, dg, dw, db, Tensor(), Tensor()};
+  }
+};
+
+std::optional<Tensor> layer_norm(const Tensor& x, const std::optional<Tensor>& gate, const std::optional<Tensor>& weight,
+                                 const std::optional<Tensor>& bias, double eps, bool save8) {
+  if (!plain(x) || !row_type(x) || !rows_in_place(x) || !(eps >= 0) || std::isinf(eps) || !plain_param(weight, x) || !plain_param(bias, x) ||
+      (weight && bias && weight->scalar_type() != bias->scalar_type()) ||
+      (gate && !(plain(*gate) && gate->scalar_type() == x.scalar_type() && gate->device() == x.device() && gate->sizes() == x.sizes() && rows_in_place(*gate))) ||
+      !plain_surroundings())
+    return std::nullopt;
+  const bool wanted = at::GradMode::is_enabled() && (x.requires_grad() || (gate && gate->requires_grad()) || (weight && weight->requires_grad()) ||
+                                                     (bias && bias->requires_grad()));
+  if (!wanted) return layer_norm_forward(x, gate.value_or(Tensor()), weight.value_or(Tensor()), bias.value_or(Tensor()), eps, false, nullptr);
+  return LayerNorm::apply(x, gate, weight, bias, eps, save8);
+}
+
+// ---- 8-bit checkpoints -----------------------------------------------------------------------------------------------------
+std::optional<std::tuple<Tensor, Tensor>> pack8(const Tensor& x) {
+  if (!plain(x) || !row_type(x) || !rows_in_place(x) || !plain_surroundings()) return std::nullopt;
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Rows r(x);
+  std::vector<int64_t> shape = x.sizes().vec();
+  shape.back() = groups(r.N);
+  const auto opt = x.options().requires_grad(false);
+  Tensor codes = at::empty(x.sizes(), opt.dtype(at::kChar)), scales = at::empty(shape, opt.dtype(at::kByte));
+  check(g_api.pack8(x.const_data_ptr(), r.ld, codes.mutable_data_ptr(), scales.mutable_data_ptr(), r.M, static_cast<int>(r.N), dtype_code(x), stream_of(x)),
+        "lab200_pack8");
+  return std::make_tuple(codes, scales);
+}
+std::optional<Tensor> unpack8(const Tensor& codes, const Tensor& scales, int dtype) {
+  if (!plain(codes) || !plain(scales) || codes.scalar_type() != at::kChar || scales.scalar_type() != at::kByte || codes.device() != scales.device() ||
+      codes.dim() < 1 || scales.dim() != codes.dim() || codes.numel() == 0 || codes.size(-1) > (1 << 30) || !codes.is_contiguous() || !scales.is_contiguous() ||
+      scales.size(-1) != groups(codes.size(-1)) || codes.sizes().slice(0, codes.dim() - 1) != scales.sizes().slice(0, codes.dim() - 1) || !plain_surroundings())
+    return std::nullopt;
+  const c10::cuda::CUDAGuard guard(codes.device());
+  const int64_t N = codes.size(-1);
+  const auto type = dtype == LAB200_F32 ? at::kFloat : dtype == LAB200_F16 ? at::kHalf : at::kBFloat16;
+  Tensor y = at::empty(codes.sizes(), codes.options().dtype(type).requires_grad(false));
+  check(g_api.unpack8(codes.const_data_ptr(), scales.const_data_ptr(), y.mutable_data_ptr(), codes.numel() / N, static_cast<int>(N), dtype, stream_of(codes)),
+        "lab200_unpack8");
+  return y;
+}
+
 }  // namespace
 
 // What this file was compiled for, for a look before it is imported (_lib.py:host_abi).
@@ -350,4 +519,7 @@ PYBIND11_MODULE(_host_ops, m) {
   m.def("decode", &decode, nogil());
   m.def("norm", &norm, nogil());
   m.def("norm_gate", &norm_gate, nogil());
+  m.def("layer_norm", &layer_norm, nogil());
+  m.def("pack8", &pack8, nogil());
+  m.def("unpack8", &unpack8, nogil());
 }

@@ -43,6 +43,10 @@ def differentiable_once(what):
 def pack_8bit(x):
     """The 8-bit checkpoint of a bf16, fp16 or fp32 tensor: (codes, scales), int8 of x's shape and uint8 with one byte for each 32
     values of the last dimension (its last group may be shorter). A group that holds an infinity or a NaN comes back as NaN. No autograd."""
+    if not torch.compiler.is_compiling():
+        r = _lib.host().pack8(x)
+        if r is not None:
+            return r
     _lib.require_cuda(x)
     dt = _lib.dtype_code(x.dtype)
     if x.dim() < 1 or x.shape[-1] < 1:
@@ -58,8 +62,12 @@ def pack_8bit(x):
 
 def unpack_8bit(codes, scales, dtype=torch.bfloat16):
     """The values that a checkpoint stands for, in codes' shape. Exact in bf16 and fp32; in fp16 rounded, and kept within +-65504."""
-    _lib.require_cuda(codes, scales)
     dt = _lib.dtype_code(dtype)
+    if not torch.compiler.is_compiling():
+        y = _lib.host().unpack8(codes, scales, dt)
+        if y is not None:
+            return y
+    _lib.require_cuda(codes, scales)
     if codes.dim() < 1 or codes.shape[-1] < 1 or not checkpoint_fits(codes, scales, codes.shape, codes.device):
         raise RuntimeError("expected int8 codes and uint8 scales with one byte for each 32 codes of the last dimension, on one device; got "
                            f"{codes.dtype} {tuple(codes.shape)} on {codes.device} and {scales.dtype} {tuple(scales.shape)} on {scales.device}")

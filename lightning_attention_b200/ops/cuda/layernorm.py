@@ -102,6 +102,11 @@ class _LayerNorm(torch.autograd.Function):
 
 
 def _apply(x, gate, weight, bias, eps, save_8bit):
+    """_LayerNorm through the native call path (csrc/host_ops.cpp) where the call has the common form, else through the class."""
+    if not torch.compiler.is_compiling():
+        y = _lib.host().layer_norm(x, gate, weight, bias, eps, save_8bit)
+        if y is not None:
+            return y
     # whether a backward pass can follow, which the class cannot see: inside it gradients are off
     wanted = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gate, weight, bias))
     return _LayerNorm.apply(x, gate, weight, bias, eps, save_8bit, wanted)

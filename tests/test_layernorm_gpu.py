@@ -377,3 +377,43 @@ def test_norm_gate_and_attention_together(cuda_lib):
     want = torch.autograd.grad(o8, (q8, k8, v8), go.view(b, n, h, d).transpose(1, 2))
     for got, ref in zip((dq, dk, dv), want):
         assert torch.equal(got, ref.transpose(1, 2))
+
+
+@pytest.mark.parametrize("gated", [False, True], ids=["norm", "gate"])
+@pytest.mark.parametrize("save_8bit", [False, True])
+@pytest.mark.parametrize("has_w,has_b", [(True, True), (True, False), (False, True), (False, False)])
+def test_native_and_python_paths_agree(cuda_lib, monkeypatch, gated, save_8bit, has_w, has_b):
+    """csrc/host_ops.cpp and the autograd class: the same results, the same tensors kept, the same refusals."""
+    from lightning_attention_b200 import _lib
+
+    x, gate, w, b, dy = inputs(33, 192, torch.bfloat16, torch.float32, gated)
+    w, b = w if has_w else None, b if has_b else None
+
+    def everything():
+        kept = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append((tuple(t.shape), t.dtype)) or t, lambda t: t):
+            y = call(x, gate, w, b, save_8bit)
+        assert torch.equal(call(x[::2], None if gate is None else gate[::2], w, b, save_8bit), y[::2])
+        leaves = [t for t in (x, gate, w, b) if t is not None]
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)], kept
+
+    native, kept = everything()
+    assert type(call(x, gate, w, b, save_8bit).grad_fn).__name__ == "CppFunction"
+    monkeypatch.setattr(_lib, "_host", _lib._NoHost())
+    python, kept_python = everything()
+    assert all(torch.equal(u, v) for u, v in zip(native, python)) and kept == kept_python
+    codes, scales = la.pack_8bit(x)
+    y = la.unpack_8bit(codes, scales)
+    monkeypatch.undo()
+    assert all(torch.equal(u, v) for u, v in zip(la.pack_8bit(x), (codes, scales))) and torch.equal(la.unpack_8bit(codes, scales), y)
+
+
+def test_no_graph_without_gradients(cuda_lib):
+    x, gate, w, b, _ = inputs(5, 64, torch.bfloat16, gated=True)
+    with torch.no_grad():
+        assert la.layer_norm(x, w, b).grad_fn is None
+    with torch.inference_mode():
+        y = la.layer_norm_sigmoid_gate(x.detach().clone(), gate.detach().clone(), w.detach().clone(), b.detach().clone())
+    assert not y.requires_grad
+    plain = [t.detach() for t in (x, w, b)]
+    assert la.layer_norm(*plain).grad_fn is None
