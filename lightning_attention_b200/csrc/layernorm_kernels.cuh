@@ -47,13 +47,18 @@ __device__ __forceinline__ void ln_param_out(void* p, int wdt, int i, float v) {
   else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
 
-// sigmoid(v) and sigmoid(-v). exp(80) is finite and sigmoid(-80) = 2e-35 nothing next to 1, so the bound changes no result and
-// keeps inf * 0 out; a NaN passes the comparison.
-__device__ __forceinline__ void ln_sigmoid(float v, float* s, float* rest) {
-  const float e = __expf(v < -80.f ? 80.f : -v);
-  *s = __fdividef(1.f, 1.f + e);
+// sigmoid(v) and sigmoid(-v) from -v / ln 2: 1 / (1 + e) and e / (1 + e), e = 2^(-v / ln 2) by the approximate instructions
+// (relative errors of 2^-22). Past 2^116 sigmoid(v) is nothing next to 1, so the bound changes no result and keeps inf * 0 out; it
+// lets a NaN pass.
+constexpr float LN_MINUS_LOG2E = -1.4426950408889634f;
+__device__ __forceinline__ void ln_sigmoid2(float arg, float* s, float* rest) {
+  float e;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(e) : "f"(arg), "f"(116.f));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(e));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(*s) : "f"(1.f + e));
   *rest = e * *s;
 }
+__device__ __forceinline__ void ln_sigmoid(float v, float* s, float* rest) { ln_sigmoid2(v * LN_MINUS_LOG2E, s, rest); }
 
 // 1 / sqrt(variance + eps) from the means of d and d^2, d = x - (the mean as computed). A NaN stays one.
 __device__ __forceinline__ float ln_rstd(float d1, float d2, float eps) {
@@ -199,9 +204,18 @@ __global__ void __launch_bounds__(256) ln_bwd_columns_kernel(const LnArgs a) {
   }
 }
 
-// ---- rows that packs of 16 bytes divide ------------------------------------------------------------------------------------
+// ---- rows in packs of 16 bytes ---------------------------------------------------------------------------------------------
 // A pack is P = 8 (16-bit) or 4 (fp32) values. Copies into shared memory run ahead (cp.async), every value comes from memory once in
 // each pass, and CTAs walk over the rows with what belongs to the columns at hand.
+//
+// ODD: rows of a contiguous tensor whose length P does not divide. The packs are those of the whole tensor: a row begins `shift` =
+// row * N mod P values into its first one and shares that and its last one with its neighbours. Teams take every so-manieth row
+// with a step that is a multiple of the shifts' period, so that a team's shift, and with it each thread's columns, stay the same.
+struct LnPackEdge { int lo, hi; };  // the values of a pack that belong to the row
+template <int P, bool ODD>
+__device__ __forceinline__ LnPackEdge ln_edge(int k, int shift, int N) {
+  return {ODD && k == 0 ? shift : 0, ODD ? min(P, N + shift - k * P) : P};
+}
 
 // Two fp32 values in one 64-bit register: the packed arithmetic of sm_100 does both at once.
 using f2 = unsigned long long;
@@ -286,13 +300,36 @@ struct LnPack {
       SrmsVec<DT>::unpack(__ldg(static_cast<const uint4*>(p) + k), f);
     }
   }
-  // The checkpoint of pack k of a row, whose group LANES adjacent lanes hold; all lanes of a warp call it, `on`: there is such a pack.
-  __device__ static void quantise(const f2* x, int8_t* codes, uint8_t* scales, int k, bool on) {
+  // Odd rows: zeros in place of the values of a pack that belong to another row, those before `lo` and from `hi` on.
+  __device__ static void cut(f2* v, int lo, int hi) {
     float f[P];
-    floats(x, f);
-    const uint32_t ex = pk_exponent(pk_group_max<LANES>(pk_abs_max<P>(f)));
+    floats(v, f);
+#pragma unroll
+    for (int j = 0; j < H; ++j)
+      v[j] = f2_of(2 * j >= lo && 2 * j < hi ? f[2 * j] : 0.f, 2 * j + 1 >= lo && 2 * j + 1 < hi ? f[2 * j + 1] : 0.f);
+  }
+  // Stores the values from `lo` to `hi` - 1 of a pack.
+  __device__ static void store_part(void* to, const f2* in, int lo, int hi) {
+    float f[P];
+    floats(in, f);
+#pragma unroll
+    for (int e = 0; e < P; ++e)
+      if (e >= lo && e < hi) SrmsElem<DT>::st(static_cast<T*>(to) + e, f[e]);
+  }
+  // Weight or bias from column c on, of which some may be no columns.
+  __device__ static void params_at(const void* p, int wdt, int c, int N, float without, f2* out) {
+    float f[P];
+#pragma unroll
+    for (int e = 0; e < P; ++e) f[e] = c + e >= 0 && c + e < N ? ln_param(p, wdt, c + e, without) : without;
+#pragma unroll
+    for (int j = 0; j < H; ++j) out[j] = f2_of(f[2 * j], f[2 * j + 1]);
+  }
+  // The checkpoint of pack k of a row (its words, and its values), whose group LANES adjacent lanes hold; all lanes of a warp call
+  // it, `on`: there is such a pack.
+  __device__ static void quantise(const uint4& words, const f2* x, int8_t* codes, uint8_t* scales, int k, bool on) {
+    const uint32_t ex = pk_pack_exponent<DT>(words);
     uint32_t w[P / 4];
-    pk_codes<P>(f, ex, w);
+    pk_pack_codes<P>(x, ex, w);
     if (on) {
       if constexpr (P == 8) reinterpret_cast<uint2*>(codes)[k] = make_uint2(w[0], w[1]);
       else reinterpret_cast<uint32_t*>(codes)[k] = w[0];
@@ -320,21 +357,25 @@ extern __shared__ __align__(16) char ln_shared[];
 // A row is a team's of T threads, V packs a thread: T a power of two up to 32 (several rows in a warp) or a multiple of 32. A warp
 // has the mean and the squares about it of its part of a row from shuffles; the parts are joined by the formula for the variance of
 // a union, behind the only barrier of a row. Each thread has places of its own in the ring of copies, so that it needs none.
+constexpr int LN_FWD_THREADS = 640;  // most of a CTA: 20 warps of up to 96 registers hide more than 16 do (32768 x 4096: 95 us, 106)
+
 struct LnFwdPlan { int T, stages; };
 
-template <int DT, int V, int G, bool GATE, bool SAVE>
-__global__ void __launch_bounds__(512) ln_fwd_kernel(const LnArgs a, const LnFwdPlan plan) {
+template <int DT, int V, int G, bool ODD, bool GATE, bool SAVE>
+__global__ void __launch_bounds__(LN_FWD_THREADS) ln_fwd_kernel(const LnArgs a, const LnFwdPlan plan) {
   using K = LnPack<DT>;
   constexpr int P = K::P, H = K::H;
-  __shared__ float4 slot[G > 32 ? 2 : 1][16];  // of a CTA's warps: mean, squares, count of their part; two halves in turn
+  static_assert(!(ODD && SAVE), "groups of 32 values do not keep to the packs of odd rows");
+  __shared__ float4 slot[G > 32 ? 2 : 1][LN_FWD_THREADS / 32];  // of a CTA's warps: mean, squares, count of their part; two halves in turn
   const int T = G <= 32 ? G : plan.T, team = threadIdx.x / T, t = threadIdx.x - team * T, lanes = blockDim.x, warp = threadIdx.x >> 5;
-  const int N = a.N, npack = N / P, ng = (N - 1) / PK_GROUP + 1, teams = lanes / T;
-  const uint32_t wplane = static_cast<uint32_t>(__cvta_generic_to_shared(ln_shared)), bplane = wplane + N * 4, ring = bplane + N * 4 + threadIdx.x * 16;
+  const int N = a.N, ng = (N - 1) / PK_GROUP + 1, teams = lanes / T;
+  const uint32_t wplane = static_cast<uint32_t>(__cvta_generic_to_shared(ln_shared)), bplane = wplane + N * 4, ring = (ODD ? wplane : bplane + N * 4) + threadIdx.x * 16;
   const uint32_t pitch = lanes * 16, stage_bytes = pitch * V * (GATE ? 2 : 1), ring_end = plan.stages * stage_bytes;
   const long long step = static_cast<long long>(gridDim.x) * teams;
   long long row = static_cast<long long>(blockIdx.x) * teams + team, ahead = row;
   long long first = G < 32 ? static_cast<long long>(blockIdx.x) * teams + (threadIdx.x & ~31) / T : row;
-  const char *x_from = static_cast<const char*>(a.x) + row * a.ldx * K::ESZ + t * 16, *g_from = static_cast<const char*>(a.gate) + row * a.ldg * K::ESZ + t * 16;
+  const int shift = ODD ? static_cast<int>(row * N % P) : 0, npack = (N + shift + P - 1) / P;
+  const char *x_from = static_cast<const char*>(a.x) + (row * a.ldx - shift) * K::ESZ + t * 16, *g_from = static_cast<const char*>(a.gate) + (row * a.ldg - shift) * K::ESZ + t * 16;
   const long long x_step = step * a.ldx * K::ESZ, g_step = step * a.ldg * K::ESZ;
   uint32_t in = 0, out = 0;
   const auto start = [&] {
@@ -342,8 +383,9 @@ __global__ void __launch_bounds__(512) ln_fwd_kernel(const LnArgs a, const LnFwd
 #pragma unroll
       for (int i = 0; i < V; ++i)
         if (t + i * T < npack) {
-          copy_async<16>(ring + in + i * pitch, x_from + i * T * 16);
-          if constexpr (GATE) copy_async<16>(ring + in + (V + i) * pitch, g_from + i * T * 16);
+          const int n = ln_edge<P, ODD>(t + i * T, shift, N).hi * K::ESZ;
+          copy_async<16>(ring + in + i * pitch, x_from + i * T * 16, n);
+          if constexpr (GATE) copy_async<16>(ring + in + (V + i) * pitch, g_from + i * T * 16, n);
         }
     }
     copies_commit();
@@ -353,20 +395,35 @@ __global__ void __launch_bounds__(512) ln_fwd_kernel(const LnArgs a, const LnFwd
     in = in + stage_bytes == ring_end ? 0 : in + stage_bytes;
   };
   for (int k = 1; k < plan.stages; ++k) start();
-  for (int k = threadIdx.x; k < npack; k += lanes) {
-    float f[P];
-    K::params(a.weight, a.wdt, a.vec_params, k, 1.f, f);
-    K::plane_put(wplane, npack, k, f);
-    K::params(a.bias, a.wdt, a.vec_params, k, 0.f, f);
-    K::plane_put(bplane, npack, k, f);
+  // weight and bias: in shared memory, or, where each team has columns of its own in a pack, in registers
+  f2 wr[ODD ? V : 1][H], br[ODD ? V : 1][H];
+  if constexpr (ODD) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      K::params_at(a.weight, a.wdt, (t + i * T) * P - shift, N, 1.f, wr[i]);
+      K::params_at(a.bias, a.wdt, (t + i * T) * P - shift, N, 0.f, br[i]);
+    }
+  } else {
+    for (int k = threadIdx.x; k < npack; k += lanes) {
+      float f[P];
+      K::params(a.weight, a.wdt, a.vec_params, k, 1.f, f);
+      K::plane_put(wplane, npack, k, f);
+      K::params(a.bias, a.wdt, a.vec_params, k, 0.f, f);
+      K::plane_put(bplane, npack, k, f);
+    }
+    __syncthreads();
   }
-  __syncthreads();
   int count = 0;  // values of a row that this warp (or sub-warp team) has
 #pragma unroll
-  for (int i = 0; i < V; ++i) count += P * min(max(npack - i * T - (G < 32 ? 0 : (t & ~31)), 0), G < 32 ? G : 32);
+  for (int i = 0; i < V; ++i) {
+    const LnPackEdge e = ln_edge<P, ODD>(t + i * T, shift, N);
+    count += t + i * T < npack ? e.hi - e.lo : 0;
+  }
+#pragma unroll
+  for (int o = (G < 32 ? G : 32) / 2; o > 0; o >>= 1) count += __shfl_xor_sync(0xffffffffu, count, o);
   const float fcount = static_cast<float>(count), inv_count = count ? 1.f / fcount : 0.f, inv_n = 1.f / static_cast<float>(N);
   int turn = 0;
-  char* y = static_cast<char*>(a.y) + row * N * K::ESZ + t * 16;
+  char* y = static_cast<char*>(a.y) + (row * N - shift) * K::ESZ + t * 16;
   const long long y_step = step * N * K::ESZ;
   for (; first < a.M; first += step, row += step, y += y_step) {
     const bool live = G >= 32 || row < a.M;
@@ -382,11 +439,13 @@ __global__ void __launch_bounds__(512) ln_fwd_kernel(const LnArgs a, const LnFwd
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       K::unpack(raw[i], v[i]);
+      const LnPackEdge e = ln_edge<P, ODD>(t + i * T, shift, N);
+      if (ODD && (e.lo > 0 || e.hi < P)) K::cut(v[i], e.lo, e.hi);
       f2 part = v[i][0];
 #pragma unroll
       for (int j = 1; j < H; ++j) part = f2_add(part, v[i][j]);
       s = f2_add(s, part);
-      if constexpr (SAVE) K::quantise(v[i], a.xcodes + row * N, a.xscales + row * ng, t + i * T, live && t + i * T < npack);
+      if constexpr (SAVE) K::quantise(raw[i], v[i], a.xcodes + row * N, a.xscales + row * ng, t + i * T, live && t + i * T < npack);
     }
     float m = f2_sum(s);
 #pragma unroll
@@ -398,8 +457,11 @@ __global__ void __launch_bounds__(512) ln_fwd_kernel(const LnArgs a, const LnFwd
     for (int i = 0; i < V; ++i) {
       f2 p1 = 0, p2 = 0;
 #pragma unroll
+      for (int j = 0; j < H; ++j) v[i][j] = f2_add(v[i][j], minus_m);
+      const LnPackEdge e = ln_edge<P, ODD>(t + i * T, shift, N);
+      if (ODD && (e.lo > 0 || e.hi < P)) K::cut(v[i], e.lo, e.hi);
+#pragma unroll
       for (int j = 0; j < H; ++j) {
-        v[i][j] = f2_add(v[i][j], minus_m);
         p1 = f2_add(p1, v[i][j]);
         p2 = f2_fma(v[i][j], v[i][j], p2);
       }
@@ -441,25 +503,32 @@ __global__ void __launch_bounds__(512) ln_fwd_kernel(const LnArgs a, const LnFwd
       const bool on = live && k < npack;
       f2 u[H];
       if constexpr (GATE) {
-        K::unpack(on ? shared16(gates + i * pitch) : make_uint4(0, 0, 0, 0), u);
-        if constexpr (SAVE) K::quantise(u, a.gcodes + row * N, a.gscales + row * ng, k, on);
+        const uint4 words = on ? shared16(gates + i * pitch) : make_uint4(0, 0, 0, 0);
+        K::unpack(words, u);
+        if constexpr (SAVE) K::quantise(words, u, a.gcodes + row * N, a.gscales + row * ng, k, on);
+#pragma unroll
+        for (int j = 0; j < H; ++j) u[j] = f2_mul(u[j], f2_all(LN_MINUS_LOG2E));
       }
       if (on) {
         f2 w[H], b[H];
-        K::plane_get(wplane, npack, k, w);
-        K::plane_get(bplane, npack, k, b);
+        if constexpr (!ODD) {
+          K::plane_get(wplane, npack, k, w);
+          K::plane_get(bplane, npack, k, b);
+        }
 #pragma unroll
         for (int j = 0; j < H; ++j) {
-          v[i][j] = f2_fma(f2_fma(v[i][j], rr, off), w[j], b[j]);
+          v[i][j] = f2_fma(f2_fma(v[i][j], rr, off), ODD ? wr[ODD ? i : 0][j] : w[j], ODD ? br[ODD ? i : 0][j] : b[j]);
           if constexpr (GATE) {
             const float2 gv = f2_get(u[j]);
             float s0, s1, rest;
-            ln_sigmoid(gv.x, &s0, &rest);
-            ln_sigmoid(gv.y, &s1, &rest);
+            ln_sigmoid2(gv.x, &s0, &rest);
+            ln_sigmoid2(gv.y, &s1, &rest);
             v[i][j] = f2_mul(v[i][j], f2_of(s0, s1));
           }
         }
-        K::store(y + i * T * 16, v[i]);
+        const LnPackEdge e = ln_edge<P, ODD>(k, shift, N);
+        if (ODD && (e.lo > 0 || e.hi < P)) K::store_part(y + i * T * 16, v[i], e.lo, e.hi);
+        else K::store(y + i * T * 16, v[i]);
       }
     }
   }
@@ -467,35 +536,36 @@ __global__ void __launch_bounds__(512) ln_fwd_kernel(const LnArgs a, const LnFwd
 }
 
 // ---- backward ----------------------------------------------------------------------------------------------------------------
-// A row is a team's of T threads, V packs a thread (E = 16 values), as in the forward pass, and a thread's columns are the same for all
-// rows: it sums dw and db in registers. The copies of a row's dy, x and gate (or their checkpoints) run some rows ahead, into
+// A row is a team's of T threads, V packs a thread (E = P V values), as in the forward pass, and a thread's columns are the same for
+// all rows: it sums dw and db in registers. The copies of a row's dy, x and gate (or their checkpoints) run some rows ahead, into
 // places that are each thread's own.
 constexpr int LN_BWD_THREADS = 512;  // most of a CTA
-constexpr int LN_PITCH = LN_BWD_THREADS * 16;  // bytes from a thread's place for one pack to that for the next
+constexpr int LN_BWD_SLOTS = LN_BWD_THREADS / 64 * 2 * 128;  // two halves of 16 warps' two sums for each team of several warps
 
 struct LnBwdPlan { int T, stages; };
 
 // What a team reads row by row: a tensor, or (SAVED) its checkpoint.
-template <int DT, int V, bool SAVED>
+// PLACE: bytes from a thread's place for one pack to that for the next.
+template <int DT, int V, bool ODD, bool SAVED>
 struct LnRows {
   using K = LnPack<DT>;
-  static constexpr int PACK = SAVED ? K::P : 16, PLACE = SAVED ? LN_PITCH / 16 * PACK : LN_PITCH, BYTES = V * PLACE;
+  static constexpr int P = K::P, PACK = SAVED ? P : 16, UNIT = PACK / P, PLACE = LN_BWD_THREADS * PACK, BYTES = V * PLACE;
   const char *p, *base;
   long long step;
-  const uint8_t* e_from;
+  const uint8_t* e_from;  // the exponents of the row
   long long e_step;
   uint32_t at;
-  uint8_t e[SAVED ? V : 1];
+  uint8_t e[SAVED ? V : 1], e2[SAVED && ODD ? V : 1];  // of a pack's group, and of the next one where the pack reaches into that
 
-  __device__ void init(const void* tensor, long long ld, const int8_t* codes, const uint8_t* scales, int N, long long row, long long rows, int t, uint32_t ring) {
+  __device__ void init(const void* tensor, long long ld, const int8_t* codes, const uint8_t* scales, int N, long long row, long long rows, int t, int shift, uint32_t ring) {
     base = SAVED ? reinterpret_cast<const char*>(codes) : static_cast<const char*>(tensor);
-    const long long pitch = SAVED ? N : ld * K::ESZ;
-    p = base + row * pitch + t * PACK;
-    step = rows * pitch;
+    const long long pitch = SAVED ? N : ld;
+    p = base + (row * pitch - shift) * UNIT + t * PACK;
+    step = rows * pitch * UNIT;
     at = ring + threadIdx.x * PACK;
     if constexpr (SAVED) {
       const int ng = (N - 1) / PK_GROUP + 1;
-      e_from = scales + row * ng + t / K::LANES;
+      e_from = scales + row * ng;
       e_step = rows * ng;
     }
   }
@@ -508,32 +578,63 @@ struct LnRows {
   }
   // FILL: teams that share a warp, of which one may have no row: its places become zero.
   template <bool FILL>
-  __device__ void start(uint32_t stage, bool live, int t, int T, int npack) {
+  __device__ void start(uint32_t stage, bool live, int t, int T, int npack, int shift, int N) {
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if (t + i * T < npack) copy_async<PACK>(stage + at + i * PLACE, FILL && !live ? base : p + i * T * PACK, FILL && !live ? 0 : PACK);
+      if (t + i * T < npack) {
+        const int n = ln_edge<P, ODD>(t + i * T, shift, N).hi * UNIT;
+        const char* from = FILL && !live ? base : p + i * T * PACK;
+        if (ODD && SAVED && n < PACK && live) {  // part of a pack of codes: whole words, and the last one's bytes
+#pragma unroll
+          for (int w = 0; w < PACK; w += 4) copy_async<4>(stage + at + i * PLACE + w, from + (w < n ? w : 0), w < n ? min(4, n - w) : 0);
+        } else {
+          copy_async<PACK>(stage + at + i * PLACE, from, FILL && !live ? 0 : n);
+        }
+      }
     p += step;
   }
-  __device__ void start_scales(bool live, int t, int T, int npack) {
+  __device__ void start_scales(bool live, int t, int T, int npack, int shift, int N) {
     if constexpr (SAVED) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) e[i] = live && t + i * T < npack ? __ldg(e_from + i * T / K::LANES) : 7;
+      for (int i = 0; i < V; ++i) {
+        const int k = t + i * T;
+        const bool on = live && k < npack;
+        e[i] = on ? __ldg(e_from + (ODD ? max(k * P - shift, 0) / PK_GROUP : k / K::LANES)) : 7;
+        if constexpr (ODD) e2[i] = on ? __ldg(e_from + min(k * P - shift + P - 1, N - 1) / PK_GROUP) : 7;
+      }
       e_from += e_step;
     }
   }
-  __device__ void get(uint32_t stage, const uint8_t* ex, f2 (*out)[K::H]) const {
+  // The values, with AFFINE times `by` plus `plus` (a checkpoint's step takes the factor in for nothing).
+  template <bool AFFINE>
+  __device__ void get(uint32_t stage, const uint8_t* ex, const uint8_t* ex2, int t, int T, int shift, float by, float plus, f2 (*out)[K::H]) const {
+    const f2 plus2 = f2_all(plus);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const uint32_t from = stage + at + i * PLACE;
       if constexpr (!SAVED) {
         K::unpack(shared16(from), out[i]);
-      } else {
-        uint32_t w[K::P / 4];
-        if constexpr (K::P == 8) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(from) : "memory");
-        else asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(from) : "memory");
-        const f2 unit = f2_all(pk_step(ex[i]));
+        if constexpr (AFFINE) {
+          const f2 by2 = f2_all(by);
 #pragma unroll
-        for (int c = 0; c < K::P; c += 2) out[i][c / 2] = f2_mul(pk_two(w[c / 4], c % 4), unit);
+          for (int j = 0; j < K::H; ++j) out[i][j] = f2_fma(out[i][j], by2, plus2);
+        }
+      } else {
+        uint32_t w[P / 4];
+        if constexpr (P == 8) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(from) : "memory");
+        else asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(from) : "memory");
+        const float unit = AFFINE ? pk_step(ex[i]) * by : pk_step(ex[i]);
+        f2 units = f2_all(unit);
+#pragma unroll
+        for (int c = 0; c < P; c += 2) {
+          if constexpr (ODD) {
+            // the next group begins with the value whose column is a multiple of 32
+            const float unit2 = AFFINE ? pk_step(ex2[i]) * by : pk_step(ex2[i]);
+            const int next = PK_GROUP - ((t + i * T) * P - shift + PK_GROUP) % PK_GROUP;
+            units = f2_of(c < next ? unit : unit2, c + 1 < next ? unit : unit2);
+          }
+          out[i][c / 2] = AFFINE ? f2_fma(pk_two(w[c / 4], c % 4), units, plus2) : f2_mul(pk_two(w[c / 4], c % 4), units);
+        }
       }
     }
   }
@@ -574,27 +675,26 @@ __device__ __forceinline__ float2 team_sum(float2 v, uint32_t slot, int t, int T
       if (T > 64) more(1, 2);
       if (T > 128) more(2, 4);
       if (T > 256) more(4, 8);
-      if (T > 512) more(8, 10);
       return make_float2(s.x + s.z, s.y + s.w);
     }
   }
 }
 
-template <int DT, int G, bool GATE, bool SAVED>
+template <int DT, int E, int G, bool ODD, bool GATE, bool SAVED>
 __global__ void __launch_bounds__(LN_BWD_THREADS) ln_bwd_kernel(const LnArgs a, const LnBwdPlan plan) {
   using K = LnPack<DT>;
-  constexpr int P = K::P, H = K::H, E = 16, V = E / P;
-  constexpr bool FILL = G < 32;
-  using In = LnRows<DT, V, SAVED>;
-  using Dy = LnRows<DT, V, false>;
-  constexpr uint32_t STAGE = Dy::BYTES + In::BYTES * (GATE ? 2 : 1), SLOTS = G > 32 ? 10 * 2 * 160 : 0;
+  constexpr int P = K::P, H = K::H, V = E / P;
+  constexpr bool FILL = G < 32, PLANES = GATE && !ODD;  // weight and bias in shared memory where registers would not do
+  using In = LnRows<DT, V, ODD, SAVED>;
+  using Dy = LnRows<DT, V, ODD, false>;
+  constexpr uint32_t STAGE = Dy::BYTES + In::BYTES * (GATE ? 2 : 1), SLOTS = G > 32 ? LN_BWD_SLOTS : 0;
   const int T = G <= 32 ? G : plan.T, team = threadIdx.x / T, t = threadIdx.x - team * T, lanes = blockDim.x, teams = lanes / T;
-  const int N = a.N, npack = N / P;
+  const int N = a.N;
   const float inv_n = 1.f / static_cast<float>(N);
-  // shared memory: the teams' slots, weight and bias (with a gate, where registers would not do), the ring
+  // shared memory: the teams' slots, weight and bias, the ring
   const uint32_t slots = static_cast<uint32_t>(__cvta_generic_to_shared(ln_shared)), wplane = slots + SLOTS, bplane = wplane + N * 4;
-  const uint32_t ring = GATE ? bplane + N * 4 : wplane, ring_end = plan.stages * STAGE;
-  uint32_t slot = slots + (G > 32 ? team * 320 : 0);
+  const uint32_t ring = PLANES ? bplane + N * 4 : wplane, ring_end = plan.stages * STAGE;
+  uint32_t slot = slots + (G > 32 ? team * 256 : 0);
   if constexpr (G > 32)
     for (int i = threadIdx.x; i < SLOTS / 4; i += lanes) asm volatile("st.shared.u32 [%0], %1;" ::"r"(slots + 4 * i), "r"(0) : "memory");
   const long long step = static_cast<long long>(gridDim.x) * teams;
@@ -602,17 +702,18 @@ __global__ void __launch_bounds__(LN_BWD_THREADS) ln_bwd_kernel(const LnArgs a, 
   const long long first = FILL ? static_cast<long long>(blockIdx.x) * teams + (threadIdx.x & ~31) / T : row;
   // rows of this team, and of the team in its warp that has most
   const int mine = row < a.M ? static_cast<int>((a.M - 1 - row) / step) + 1 : 0, most = first < a.M ? static_cast<int>((a.M - 1 - first) / step) + 1 : 0;
+  const int shift = ODD ? static_cast<int>(row * N % P) : 0, npack = (N + shift + P - 1) / P;
   In x, g;
   Dy dy;
-  dy.init(a.dy, a.lddy, nullptr, nullptr, N, row, step, t, ring);
-  x.init(a.x, a.ldx, a.xcodes, a.xscales, N, row, step, t, ring + Dy::BYTES);
-  if constexpr (GATE) g.init(a.gate, a.ldg, a.gcodes, a.gscales, N, row, step, t, ring + Dy::BYTES + In::BYTES);
+  dy.init(a.dy, a.lddy, nullptr, nullptr, N, row, step, t, shift, ring);
+  x.init(a.x, a.ldx, a.xcodes, a.xscales, N, row, step, t, shift, ring + Dy::BYTES);
+  if constexpr (GATE) g.init(a.gate, a.ldg, a.gcodes, a.gscales, N, row, step, t, shift, ring + Dy::BYTES + In::BYTES);
   uint32_t in = 0, out = 0;
   const auto start = [&](int n) {
     if (FILL || n < mine) {
-      dy.template start<FILL>(in, n < mine, t, T, npack);
-      x.template start<FILL>(in, n < mine, t, T, npack);
-      if constexpr (GATE) g.template start<FILL>(in, n < mine, t, T, npack);
+      dy.template start<FILL>(in, n < mine, t, T, npack, shift, N);
+      x.template start<FILL>(in, n < mine, t, T, npack, shift, N);
+      if constexpr (GATE) g.template start<FILL>(in, n < mine, t, T, npack, shift, N);
     }
     copies_commit();
     in = in + STAGE == ring_end ? 0 : in + STAGE;
@@ -622,8 +723,8 @@ __global__ void __launch_bounds__(LN_BWD_THREADS) ln_bwd_kernel(const LnArgs a, 
   const auto start_small = [&](int n) {
     st_next = n < mine ? __ldg(st_from) : make_float2(0.f, 0.f);
     st_from += step;
-    x.start_scales(n < mine, t, T, npack);
-    if constexpr (GATE) g.start_scales(n < mine, t, T, npack);
+    x.start_scales(n < mine, t, T, npack, shift, N);
+    if constexpr (GATE) g.start_scales(n < mine, t, T, npack, shift, N);
   };
   for (int k = 0; k < plan.stages; ++k) {
     dy.clear(k * STAGE);
@@ -632,11 +733,14 @@ __global__ void __launch_bounds__(LN_BWD_THREADS) ln_bwd_kernel(const LnArgs a, 
   }
   for (int k = 1; k < plan.stages; ++k) start(k - 1);
   start_small(0);
-  f2 w[GATE ? 1 : V][H], dw[V][H], db[V][H];
+  f2 w[PLANES ? 1 : V][H], b[GATE && !PLANES ? V : 1][H], dw[V][H], db[V][H];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int k = t + i * T;
-    if constexpr (!GATE) {
+    if constexpr (ODD) {
+      K::params_at(a.weight, a.wdt, k * P - shift, N, 1.f, w[i]);
+      if constexpr (GATE) K::params_at(a.bias, a.wdt, k * P - shift, N, 0.f, b[i]);
+    } else if constexpr (!PLANES) {
       float f[P];
       K::params(k < npack ? a.weight : nullptr, a.wdt, a.vec_params, k, 1.f, f);
 #pragma unroll
@@ -645,7 +749,7 @@ __global__ void __launch_bounds__(LN_BWD_THREADS) ln_bwd_kernel(const LnArgs a, 
 #pragma unroll
     for (int j = 0; j < H; ++j) dw[i][j] = db[i][j] = 0;
   }
-  if constexpr (GATE)
+  if constexpr (PLANES)
     for (int k = threadIdx.x; k < npack; k += lanes) {
       float f[P];
       K::params(a.weight, a.wdt, a.vec_params, k, 1.f, f);
@@ -653,49 +757,67 @@ __global__ void __launch_bounds__(LN_BWD_THREADS) ln_bwd_kernel(const LnArgs a, 
       K::params(a.bias, a.wdt, a.vec_params, k, 0.f, f);
       K::plane_put(bplane, npack, k, f);
     }
-  if constexpr (GATE || G > 32) __syncthreads();
-  char *dx = static_cast<char*>(a.dx) + row * N * K::ESZ + t * 16, *dg = static_cast<char*>(a.dgate) + row * N * K::ESZ + t * 16;
+  if constexpr (PLANES || G > 32) __syncthreads();
+  char *dx = static_cast<char*>(a.dx) + (row * N - shift) * K::ESZ + t * 16, *dg = static_cast<char*>(a.dgate) + (row * N - shift) * K::ESZ + t * 16;
   const long long out_step = step * N * K::ESZ;
   for (int n = 0; n < most; ++n, dx += out_step, dg += out_step) {
     const bool live = !FILL || n < mine;
     copies_wait(plan.stages);
     const float2 st = st_next;
-    uint8_t ex[SAVED ? V : 1], eg[SAVED && GATE ? V : 1];
+    uint8_t ex[SAVED ? V : 1], eg[SAVED && GATE ? V : 1], ex2[SAVED && ODD ? V : 1], eg2[SAVED && GATE && ODD ? V : 1];
     if constexpr (SAVED) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         ex[i] = x.e[i];
+        if constexpr (ODD) ex2[i] = x.e2[i];
         if constexpr (GATE) eg[i] = g.e[i];
+        if constexpr (GATE && ODD) eg2[i] = g.e2[i];
       }
     }
     f2 xh[V][H], s[V][H];
-    dy.get(out, nullptr, s);
-    x.get(out, ex, xh);
-    const f2 rr = f2_all(st.y), off = f2_all(-st.x * st.y);
+    dy.template get<false>(out, nullptr, nullptr, t, T, shift, 1.f, 0.f, s);
+    x.template get<true>(out, ex, ex2, t, T, shift, st.y, -st.x * st.y, xh);
+    if constexpr (ODD) {
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-#pragma unroll
-      for (int j = 0; j < H; ++j) xh[i][j] = f2_fma(xh[i][j], rr, off);
+      for (int i = 0; i < V; ++i) {
+        const LnPackEdge e = ln_edge<P, ODD>(t + i * T, shift, N);
+        if (e.lo > 0 || e.hi < P) {
+          K::cut(s[i], e.lo, e.hi);
+          K::cut(xh[i], e.lo, e.hi);
+        }
+      }
+    }
+    const f2 rr = f2_all(st.y);
     if constexpr (GATE) {
       f2 u[V][H];
-      g.get(out, eg, u);
+      g.template get<true>(out, eg, eg2, t, T, shift, LN_MINUS_LOG2E, 0.f, u);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const int k = t + i * T;
         if (k < npack) {
           f2 wk[H], bk[H];
-          K::plane_get(wplane, npack, k, wk);
-          K::plane_get(bplane, npack, k, bk);
+          if constexpr (PLANES) {
+            K::plane_get(wplane, npack, k, wk);
+            K::plane_get(bplane, npack, k, bk);
+          } else {
+#pragma unroll
+            for (int j = 0; j < H; ++j) { wk[j] = w[i][j]; bk[j] = b[i][j]; }
+          }
+          const LnPackEdge e = ln_edge<P, ODD>(k, shift, N);
+          if (ODD && (e.lo > 0 || e.hi < P)) K::cut(u[i], e.lo, e.hi);
 #pragma unroll
           for (int j = 0; j < H; ++j) {
             const float2 gv = f2_get(u[i][j]);
             float s0, s1, r0, r1;
-            ln_sigmoid(gv.x, &s0, &r0);
-            ln_sigmoid(gv.y, &s1, &r1);
+            ln_sigmoid2(gv.x, &s0, &r0);
+            ln_sigmoid2(gv.y, &s1, &r1);
             s[i][j] = f2_mul(s[i][j], f2_of(s0, s1));
             u[i][j] = f2_mul(f2_mul(s[i][j], f2_fma(xh[i][j], wk[j], bk[j])), f2_of(r0, r1));
           }
-          if (a.dgate && live) K::store(dg + i * T * 16, u[i]);
+          if (a.dgate && live) {
+            if (ODD && (e.lo > 0 || e.hi < P)) K::store_part(dg + i * T * 16, u[i], e.lo, e.hi);
+            else K::store(dg + i * T * 16, u[i]);
+          }
         }
       }
     }
@@ -706,14 +828,14 @@ __global__ void __launch_bounds__(LN_BWD_THREADS) ln_bwd_kernel(const LnArgs a, 
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       f2 wk[H];
-      if constexpr (GATE) {
+      if constexpr (PLANES) {
 #pragma unroll
         for (int j = 0; j < H; ++j) wk[j] = 0;
         if (t + i * T < npack) K::plane_get(wplane, npack, t + i * T, wk);
       }
 #pragma unroll
       for (int j = 0; j < H; ++j) {
-        const f2 wij = GATE ? wk[j] : w[GATE ? 0 : i][j];
+        const f2 wij = PLANES ? wk[j] : w[PLANES ? 0 : i][j];
         db[i][j] = f2_add(db[i][j], s[i][j]);
         const f2 p = f2_mul(s[i][j], xh[i][j]);
         dw[i][j] = f2_add(dw[i][j], p);
@@ -729,18 +851,46 @@ __global__ void __launch_bounds__(LN_BWD_THREADS) ln_bwd_kernel(const LnArgs a, 
       for (int i = 0; i < V; ++i) {
 #pragma unroll
         for (int j = 0; j < H; ++j) s[i][j] = f2_fma(s[i][j], rr, f2_fma(xh[i][j], k2, k1));
-        if (t + i * T < npack) K::store(dx + i * T * 16, s[i]);
+        const LnPackEdge e = ln_edge<P, ODD>(t + i * T, shift, N);
+        if (t + i * T < npack) {
+          if (ODD && (e.lo > 0 || e.hi < P)) K::store_part(dx + i * T * 16, s[i], e.lo, e.hi);
+          else K::store(dx + i * T * 16, s[i]);
+        }
       }
     }
-    if constexpr (G > 32) slot = slots + team * 320 + ((n & 1) ? 0 : 160);
+    if constexpr (G > 32) slot = slots + team * 256 + ((n & 1) ? 0 : 128);
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   if (!a.partial) return;
+  float* sums = reinterpret_cast<float*>(ln_shared);
+  if constexpr (ODD) {
+    // The CTA's part of dw and db: teams have columns of their own in a pack, so their sums meet by column in shared memory, one
+    // team after the other.
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      for (int k = 0; k < teams; ++k) {
+        __syncthreads();
+        if (team == k)
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            float f[P];
+            K::floats(which ? db[i] : dw[i], f);
+#pragma unroll
+            for (int e = 0; e < P; ++e) {
+              const int col = (t + i * T) * P - shift + e;
+              if (col >= 0 && col < N) sums[col] = k ? sums[col] + f[e] : f[e];
+            }
+          }
+      }
+      __syncthreads();
+      for (int col = threadIdx.x; col < N; col += lanes) a.partial[(static_cast<size_t>(blockIdx.x) * 2 + which) * N + col] = sums[col];
+    }
+    return;
+  }
   // The CTA's part of dw and db: its teams' (for rows within a warp, its warps') sums in their order, through shared memory.
   constexpr int LW = G < 32 ? G : 32;
   const int span = G <= 32 ? 32 : T, TT = G <= 32 ? LW : T, units = lanes / span, unit = threadIdx.x / span, tt = threadIdx.x - unit * span;
   const bool holds = tt < TT;
-  float* sums = reinterpret_cast<float*>(ln_shared);
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     float acc[E];

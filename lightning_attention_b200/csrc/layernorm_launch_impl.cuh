@@ -5,13 +5,17 @@ namespace lab200 {
 
 constexpr int LN_SHARED = 232448;  // bytes of shared memory that a CTA may have
 
-// Whether packs of 16 bytes divide every row of every tensor of the call, and whole words its checkpoints.
-inline bool ln_packs(const LnArgs& a, int esz) {
-  uintptr_t bits = static_cast<uintptr_t>(a.N) * esz;
+enum LnRowKind { LN_ANY, LN_PACKS, LN_ODD };
+
+// How a call's rows may be read: in packs of 16 bytes that divide every row of every tensor (and words that divide its checkpoints);
+// in the packs of whole contiguous tensors; element by element.
+inline LnRowKind ln_kind(const LnArgs& a, int esz) {
+  uintptr_t bits = 0;  // of pointers and row strides
+  bool contiguous = true;
   const auto tensor = [&](const void* p, long long ld) {
     if (!p) return;
     bits |= reinterpret_cast<uintptr_t>(p);
-    if (a.M > 1) bits |= static_cast<uintptr_t>(ld) * esz;
+    if (a.M > 1 && ld != a.N) bits |= static_cast<uintptr_t>(ld) * esz, contiguous = false;
   };
   tensor(a.x, a.ldx);
   tensor(a.gate, a.ldg);
@@ -20,8 +24,22 @@ inline bool ln_packs(const LnArgs& a, int esz) {
   tensor(a.dx, a.N);
   tensor(a.dgate, a.N);
   const uintptr_t codes = reinterpret_cast<uintptr_t>(a.xcodes) | reinterpret_cast<uintptr_t>(a.gcodes);
-  const uintptr_t scales = reinterpret_cast<uintptr_t>(a.xscales) | reinterpret_cast<uintptr_t>(a.gscales);
-  return bits % 16 == 0 && codes % (16 / esz) == 0 && scales % 4 == 0;
+  if (bits % 16 || codes % (16 / esz)) return LN_ANY;
+  return a.N % (16 / esz) == 0 ? LN_PACKS : contiguous ? LN_ODD : LN_ANY;
+}
+
+// Rows after which the shifts of odd rows repeat.
+inline int ln_period(int N, int P) {
+  int q = P;
+  while (q > 1 && (static_cast<long long>(N) * (q / 2)) % P == 0) q /= 2;
+  return q;
+}
+// `ctas` of `teams` each, a few more or (past `most`) fewer, so that all teams together are a multiple of the period.
+inline long long ln_even(long long ctas, long long most, int teams, int period) {
+  int unit = period;
+  while (unit > 1 && (static_cast<long long>(unit / 2) * teams) % period == 0) unit /= 2;
+  ctas = (ctas + unit - 1) / unit * unit;
+  return ctas <= most ? ctas : most / unit * unit > 0 ? most / unit * unit : unit;
 }
 
 template <class Kern, class Plan>
@@ -42,76 +60,90 @@ cudaError_t ln_fwd_any(const LnArgs& a, LnPlace at) {
   return cudaGetLastError();
 }
 
-template <int DT, int V, int G>
+template <int DT, int V, int G, bool ODD>
 cudaError_t ln_fwd_team(const LnArgs& a, LnPlace at, int T) {
   const bool gate = a.gate, save = a.xcodes;
-  const int cta = 512 / T * T, stage = cta * 16 * V * (gate ? 2 : 1);
-  const long long teams = cta / T, ctas = (a.M + teams - 1) / teams;
-  const size_t planes = static_cast<size_t>(a.N) * 8;
-  int stages = static_cast<int>((LN_SHARED - 1024 - planes) / stage);
+  const int teams = LN_FWD_THREADS / T, cta = teams * T, stage = cta * 16 * V * (gate ? 2 : 1);
+  const size_t planes = ODD ? 0 : static_cast<size_t>(a.N) * 8;
+  int stages = planes > LN_SHARED - 2048 ? 0 : static_cast<int>((LN_SHARED - 2048 - planes) / stage);
   if (stages < 2) return ln_fwd_any<DT>(a, at);
   stages = stages > 4 ? 4 : stages;
   const LnFwdPlan plan{T, stages};
   const size_t shared = planes + static_cast<size_t>(stages) * stage;
-  const unsigned grid = ln_capped(ctas, at.sms);
-  if (gate) return save ? ln_launch(ln_fwd_kernel<DT, V, G, true, true>, grid, cta, shared, at.st, a, plan)
-                        : ln_launch(ln_fwd_kernel<DT, V, G, true, false>, grid, cta, shared, at.st, a, plan);
-  return save ? ln_launch(ln_fwd_kernel<DT, V, G, false, true>, grid, cta, shared, at.st, a, plan)
-              : ln_launch(ln_fwd_kernel<DT, V, G, false, false>, grid, cta, shared, at.st, a, plan);
+  const unsigned grid = static_cast<unsigned>(ln_even((a.M + teams - 1) / teams, at.sms, teams, ODD ? ln_period(a.N, LnPack<DT>::P) : 1));
+  if constexpr (ODD) {
+    return gate ? ln_launch(ln_fwd_kernel<DT, V, G, true, true, false>, grid, cta, shared, at.st, a, plan)
+                : ln_launch(ln_fwd_kernel<DT, V, G, true, false, false>, grid, cta, shared, at.st, a, plan);
+  } else {
+    if (gate) return save ? ln_launch(ln_fwd_kernel<DT, V, G, false, true, true>, grid, cta, shared, at.st, a, plan)
+                          : ln_launch(ln_fwd_kernel<DT, V, G, false, true, false>, grid, cta, shared, at.st, a, plan);
+    return save ? ln_launch(ln_fwd_kernel<DT, V, G, false, false, true>, grid, cta, shared, at.st, a, plan)
+                : ln_launch(ln_fwd_kernel<DT, V, G, false, false, false>, grid, cta, shared, at.st, a, plan);
+  }
 }
 
 template <int DT>
 cudaError_t ln_fwd(const LnArgs& a, LnPlace at) {
   using K = LnPack<DT>;
+  const LnRowKind kind = ln_kind(a, K::ESZ);
+  const auto team = [](int npack, int v) { return (npack + v * 32 - 1) / (v * 32) * 32; };
+  if (kind == LN_ODD && !a.xcodes) {
+    constexpr int V = 16 / K::P;
+    const int npack = (a.N + 2 * K::P - 2) / K::P;  // of the row that begins last in its first pack
+    if (npack <= 8 * V) return ln_fwd_team<DT, V, 8, true>(a, at, 8);
+    if (npack <= 32 * V) return ln_fwd_team<DT, V, 32, true>(a, at, 32);
+    if (npack <= 512 * V) return ln_fwd_team<DT, V, 64, true>(a, at, team(npack, V));
+  }
   const int npack = a.N / K::P;
-  if (!ln_packs(a, K::ESZ) || npack > 512 * 4) return ln_fwd_any<DT>(a, at);
-  const auto team = [&](int v) { return (npack + v * 32 - 1) / (v * 32) * 32; };
-  if (npack <= 512 && a.M * team(4) < 148 * 256) return npack <= 32 ? ln_fwd_team<DT, 1, 32>(a, at, 32) : ln_fwd_team<DT, 1, 64>(a, at, team(1));
-  if (npack <= 16 && K::LANES <= 4) return ln_fwd_team<DT, 4, 4>(a, at, 4);
-  if (npack <= 32) return ln_fwd_team<DT, 4, 8>(a, at, 8);
-  if (npack <= 64) return ln_fwd_team<DT, 4, 16>(a, at, 16);
-  if (npack <= 128) return ln_fwd_team<DT, 4, 32>(a, at, 32);
-  return ln_fwd_team<DT, 4, 64>(a, at, team(4));
+  if (kind != LN_PACKS || npack > 512 * 4) return ln_fwd_any<DT>(a, at);
+  if (npack <= 512 && a.M * team(npack, 4) < 148 * 256)
+    return npack <= 32 ? ln_fwd_team<DT, 1, 32, false>(a, at, 32) : ln_fwd_team<DT, 1, 64, false>(a, at, team(npack, 1));
+  if (npack <= 16 && K::LANES <= 4) return ln_fwd_team<DT, 4, 4, false>(a, at, 4);
+  if (npack <= 32) return ln_fwd_team<DT, 4, 8, false>(a, at, 8);
+  if (npack <= 64) return ln_fwd_team<DT, 4, 16, false>(a, at, 16);
+  if (npack <= 128) return ln_fwd_team<DT, 4, 32, false>(a, at, 32);
+  return ln_fwd_team<DT, 4, 64, false>(a, at, team(npack, 4));
 }
 
-struct LnBwdLaunch { LnBwdPlan plan; int G, cta; size_t shared; int parts; };
+struct LnBwdLaunch { LnBwdPlan plan; LnRowKind kind; int G, cta; size_t shared; int parts; };
 
 // False: no kernel that keeps rows in registers takes the call.
 template <int DT>
 bool ln_bwd_plan(const LnArgs& a, LnPlace at, LnBwdLaunch* l) {
   using K = LnPack<DT>;
-  constexpr int E = 16, V = E / K::P;
   const bool gate = a.gate || a.gcodes, saved = a.xcodes;
-  const int npack = a.N / K::P;
-  if (!ln_packs(a, K::ESZ) || npack > LN_BWD_THREADS * V) return false;
-  const int G = npack <= 8 * V ? 8 : npack <= 16 * V ? 16 : npack <= 32 * V ? 32 : 64;
-  const int T = G <= 32 ? G : (npack + V * 32 - 1) / (V * 32) * 32;
-  l->G = G;
-  // up to 512 threads; one team more where that is a good part of a CTA's
-  int teams = 512 / T;
-  if ((teams + 1) * T <= LN_BWD_THREADS && teams <= 1) ++teams;
+  l->kind = ln_kind(a, K::ESZ);
+  if (l->kind == LN_ANY) return false;
+  const bool odd = l->kind == LN_ODD;
+  const int npack = odd ? (a.N + 2 * K::P - 2) / K::P : a.N / K::P;  // odd rows: of the one that begins last in its first pack
+  const auto team = [&](int e) { return (npack + e / K::P * 32 - 1) / (e / K::P * 32) * 32; };
+  const int E = odd && gate ? 8 : 16, V = E / K::P;
+  if (npack > LN_BWD_THREADS * V) return false;
+  l->G = npack <= 8 * V ? 8 : npack <= 16 * V ? 16 : npack <= 32 * V ? 32 : 64;
+  const int T = l->G <= 32 ? l->G : team(E), teams = LN_BWD_THREADS / T;
   l->cta = teams * T;
-  const size_t in = static_cast<size_t>(V) * LN_PITCH / 16 * (saved ? K::P : 16), stage = static_cast<size_t>(V) * LN_PITCH + in * (gate ? 2 : 1);
-  const size_t fixed = (G > 32 ? 10 * 2 * 160 : 0) + (gate ? static_cast<size_t>(a.N) * 8 : 0);
-  const int units = l->cta / (G <= 32 ? 32 : T);
-  const size_t sums = static_cast<size_t>(units - 1) * E * T * 4;
-  const int stages = static_cast<int>((LN_SHARED - fixed) / stage);
-  if (fixed > LN_SHARED || stages < 2) return false;
+  const size_t in = static_cast<size_t>(V) * LN_BWD_THREADS * (saved ? K::P : 16), stage = static_cast<size_t>(V) * LN_BWD_THREADS * 16 + in * (gate ? 2 : 1);
+  const size_t fixed = (l->G > 32 ? LN_BWD_SLOTS : 0) + (gate && !odd ? static_cast<size_t>(a.N) * 8 : 0);
+  const int units = l->cta / (l->G <= 32 ? 32 : T);
+  const size_t sums = odd ? static_cast<size_t>(a.N) * 4 : static_cast<size_t>(units - 1) * E * T * 4;
+  const int stages = fixed > LN_SHARED ? 0 : static_cast<int>((LN_SHARED - fixed) / stage);
+  if (stages < 2) return false;
   l->plan = {T, stages > 4 ? 4 : stages};
   l->shared = fixed + l->plan.stages * stage;
   if (sums > l->shared) l->shared = sums;
-  const long long ctas = (a.M + teams - 1) / teams;
-  l->parts = static_cast<int>(ln_capped(ctas, at.sms < LN_MAX_PARTS ? at.sms : LN_MAX_PARTS));
-  return (a.M + teams - 1) / teams / l->parts < (1 << 30);
+  const long long most = at.sms < LN_MAX_PARTS ? at.sms : LN_MAX_PARTS;
+  l->parts = static_cast<int>(ln_even((a.M + teams - 1) / teams, most, teams, odd ? ln_period(a.N, K::P) : 1));
+  return a.M / teams / l->parts < (1 << 30);
 }
 
-template <int DT, int G>
+template <int DT, int G, bool ODD>
 cudaError_t ln_bwd_team(const LnArgs& a, LnPlace at, const LnBwdLaunch& l) {
   const bool gate = a.gate || a.gcodes, saved = a.xcodes;
-  if (gate) return saved ? ln_launch(ln_bwd_kernel<DT, G, true, true>, l.parts, l.cta, l.shared, at.st, a, l.plan)
-                         : ln_launch(ln_bwd_kernel<DT, G, true, false>, l.parts, l.cta, l.shared, at.st, a, l.plan);
-  return saved ? ln_launch(ln_bwd_kernel<DT, G, false, true>, l.parts, l.cta, l.shared, at.st, a, l.plan)
-               : ln_launch(ln_bwd_kernel<DT, G, false, false>, l.parts, l.cta, l.shared, at.st, a, l.plan);
+  constexpr int E = 16, EG = ODD ? 8 : 16;
+  if (gate) return saved ? ln_launch(ln_bwd_kernel<DT, EG, G, ODD, true, true>, l.parts, l.cta, l.shared, at.st, a, l.plan)
+                         : ln_launch(ln_bwd_kernel<DT, EG, G, ODD, true, false>, l.parts, l.cta, l.shared, at.st, a, l.plan);
+  return saved ? ln_launch(ln_bwd_kernel<DT, E, G, ODD, false, true>, l.parts, l.cta, l.shared, at.st, a, l.plan)
+               : ln_launch(ln_bwd_kernel<DT, E, G, ODD, false, false>, l.parts, l.cta, l.shared, at.st, a, l.plan);
 }
 
 template <int DT>
@@ -123,8 +155,13 @@ int ln_bwd_parts(const LnArgs& a, LnPlace at) {
 template <int DT>
 cudaError_t ln_bwd(LnArgs a, LnPlace at) {
   LnBwdLaunch l;
-  if (ln_bwd_plan<DT>(a, at, &l))
-    return l.G == 8 ? ln_bwd_team<DT, 8>(a, at, l) : l.G == 16 ? ln_bwd_team<DT, 16>(a, at, l) : l.G == 32 ? ln_bwd_team<DT, 32>(a, at, l) : ln_bwd_team<DT, 64>(a, at, l);
+  if (ln_bwd_plan<DT>(a, at, &l)) {
+    if (l.kind == LN_ODD)
+      return l.G == 8 ? ln_bwd_team<DT, 8, true>(a, at, l) : l.G == 16 ? ln_bwd_team<DT, 16, true>(a, at, l)
+           : l.G == 32 ? ln_bwd_team<DT, 32, true>(a, at, l) : ln_bwd_team<DT, 64, true>(a, at, l);
+    return l.G == 8 ? ln_bwd_team<DT, 8, false>(a, at, l) : l.G == 16 ? ln_bwd_team<DT, 16, false>(a, at, l)
+         : l.G == 32 ? ln_bwd_team<DT, 32, false>(a, at, l) : ln_bwd_team<DT, 64, false>(a, at, l);
+  }
   if (a.dx || a.dgate) {
     ln_bwd_any_kernel<DT><<<ln_capped(a.M, 1 << 20), 256, 0, at.st>>>(a);
     count_launch();

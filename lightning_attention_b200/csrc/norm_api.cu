@@ -103,12 +103,20 @@ int lab200_layernorm_fwd(const void* x, long long ldx, const void* gate, long lo
   if (reinterpret_cast<uintptr_t>(stats) & 7) return LAB200_ERR_ALIGN;
   a.vec_params = aligned_params(a);
   const LnPlace at{sm_count(), static_cast<cudaStream_t>(stream)};
+  // groups of 32 values do not keep to the packs of odd rows: those are checkpointed on their own
+  if (xcodes && N % (dtype == LAB200_F32 ? 4 : 8)) {
+    int rc = lab200_pack8(x, ldx, xcodes, xscales, M, N, dtype, stream);
+    if (rc == LAB200_OK && gate) rc = lab200_pack8(gate, ldg, gcodes, gscales, M, N, dtype, stream);
+    if (rc != LAB200_OK) return rc;
+    a.xcodes = a.gcodes = nullptr;
+    a.xscales = a.gscales = nullptr;
+  }
   const cudaError_t rc = dtype == LAB200_F32 ? ln_fwd<SRMS_F32>(a, at) : dtype == LAB200_F16 ? ln_fwd<SRMS_F16>(a, at) : ln_fwd<SRMS_BF16>(a, at);
   return rc == cudaSuccess ? LAB200_OK : LAB200_ERR_CUDA;
 }
 
 size_t lab200_layernorm_bwd_workspace_bytes(long long M, int N) {
-  return N < 1 || M < 1 ? 0 : static_cast<size_t>(M < LN_MAX_PARTS ? M : LN_MAX_PARTS) * 2 * N * sizeof(float);
+  return N < 1 || M < 1 ? 0 : static_cast<size_t>(M + 8 < LN_MAX_PARTS ? M + 8 : LN_MAX_PARTS) * 2 * N * sizeof(float);
 }
 
 int lab200_layernorm_bwd(const void* x, long long ldx, const void* gate, long long ldg, const void* xcodes, const void* xscales, const void* gcodes,

@@ -33,41 +33,48 @@ __device__ __forceinline__ float pk_bound(float v) {
   return v;
 }
 
-// The largest magnitude of P values, as bits; a NaN among them wins.
-template <int P>
-__device__ __forceinline__ uint32_t pk_abs_max(const float* f) {
-  float m = fabsf(f[0]);
+// Exponent byte of the group of which this lane has a pack of 16 bytes and adjacent lanes the rest (4 lanes of 16-bit values, 8 of
+// fp32); all lanes of a warp call it. Magnitudes of each type compare as whole numbers, infinities and NaN above the rest; 16-bit
+// ones two at a time.
+template <int DT>
+__device__ __forceinline__ uint32_t pk_pack_exponent(const uint4& w) {
+  constexpr uint32_t ALL = 0xffffffffu;
+  if constexpr (DT == SRMS_F32) {
+    uint32_t m = max(max(w.x & 0x7fffffffu, w.y & 0x7fffffffu), max(w.z & 0x7fffffffu, w.w & 0x7fffffffu));
 #pragma unroll
-  for (int e = 1; e < P; ++e) asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(m), "f"(fabsf(f[e])));
-  return __float_as_uint(m);
-}
-// Its maximum over LANES adjacent lanes, which hold one group.
-template <int LANES>
-__device__ __forceinline__ uint32_t pk_group_max(uint32_t bits) {
-  if constexpr (LANES == 32) return __reduce_max_sync(0xffffffffu, bits);
+    for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(ALL, m, o));
+    return pk_exponent(m);
+  } else {
+    uint32_t m = __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
 #pragma unroll
-  for (int o = 1; o < LANES; o <<= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
-  return bits;
+    for (int o = 1; o < 4; o <<= 1) m = __vmaxu2(m, __shfl_xor_sync(ALL, m, o));
+    m = max(m & 0xffffu, m >> 16);
+    if constexpr (DT == SRMS_BF16) return pk_exponent(m << 16);
+    return pk_exponent(__float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m)))));
+  }
 }
-// P codes, four to a word. Adding 1.5 * 2^23 rounds to a whole number, to nearest even, and leaves it in the low byte: exact, as
-// x * inv is. Groups of E = 254 (whose codes may have to be held at 127) and 255 take the checked way.
+// P codes, four to a word, from pairs of fp32 values. Adding 1.5 * 2^23 rounds to a whole number, to nearest even, and leaves it in the
+// low byte: exact, as x * inv is. Groups of E = 254 (whose codes may have to be held at 127) and 255 take the checked way.
 template <int P>
-__device__ __forceinline__ void pk_codes(const float* f, uint32_t e, uint32_t* w) {
+__device__ __forceinline__ void pk_pack_codes(const unsigned long long* x, uint32_t e, uint32_t* w) {
   const float inv = pk_inv_step(e);
   uint32_t c[P];
   if (e < 254u) {
 #pragma unroll
-    for (int i = 0; i < P; ++i) c[i] = __float_as_uint(fmaf(f[i], inv, 12582912.f));
+    for (int i = 0; i < P; i += 2)
+      asm("{ .reg .b64 s, m, r; mov.b64 s, {%3, %3}; mov.b64 m, {%4, %4}; fma.rn.f32x2 r, %2, s, m; mov.b64 {%0, %1}, r; }"
+          : "=r"(c[i]), "=r"(c[i + 1]) : "l"(x[i / 2]), "r"(__float_as_uint(inv)), "r"(__float_as_uint(12582912.f)));
   } else {
 #pragma unroll
-    for (int i = 0; i < P; ++i) c[i] = static_cast<uint32_t>(pk_code(f[i], inv));
+    for (int i = 0; i < P; i += 2) {
+      float lo, hi;
+      asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x[i / 2]));
+      c[i] = static_cast<uint32_t>(pk_code(lo, inv));
+      c[i + 1] = static_cast<uint32_t>(pk_code(hi, inv));
+    }
   }
-  if constexpr (P == 1) {
-    w[0] = c[0];
-  } else {
 #pragma unroll
-    for (int i = 0; i < P; i += 4) w[i / 4] = __byte_perm(__byte_perm(c[i], c[i + 1], 0x0040), __byte_perm(c[i + 2], c[i + 3], 0x0040), 0x5410);
-  }
+  for (int i = 0; i < P; i += 4) w[i / 4] = __byte_perm(__byte_perm(c[i], c[i + 1], 0x0040), __byte_perm(c[i + 2], c[i + 3], 0x0040), 0x5410);
 }
 // Two adjacent codes of a word as fp32 values: a byte b, moved by 128, in the low byte of 2^23 makes 2^23 + b + 128.
 __device__ __forceinline__ unsigned long long pk_two(uint32_t w, int e) {
@@ -120,9 +127,12 @@ pack8_kernel(const void* __restrict__ x_, long long ldx, int8_t* __restrict__ co
       const long long k = k0 + 32 * i;
       float f[P];
       SrmsVec<DT>::unpack(v[i].q[0], f);
-      const uint32_t e = pk_exponent(pk_group_max<LANES>(pk_abs_max<P>(f)));
+      unsigned long long two[P / 2];
+#pragma unroll
+      for (int c = 0; c < P; c += 2) asm("mov.b64 %0, {%1, %2};" : "=l"(two[c / 2]) : "f"(f[c]), "f"(f[c + 1]));
+      const uint32_t e = pk_pack_exponent<DT>(v[i].q[0]);
       uint32_t w[P / 4];
-      pk_codes<P>(f, e, w);
+      pk_pack_codes<P>(two, e, w);
       if (k < r.npack) {
         if constexpr (P == 8) reinterpret_cast<uint2*>(to)[k] = make_uint2(w[0], w[1]);
         else to[k] = w[0];
