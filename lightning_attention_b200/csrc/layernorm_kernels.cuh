@@ -227,9 +227,14 @@ __device__ __forceinline__ f2 f2_mul(f2 a, f2 b) { f2 r; asm("mul.rn.f32x2 %0, %
 __device__ __forceinline__ f2 f2_fma(f2 a, f2 b, f2 c) { f2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
 __device__ __forceinline__ float f2_sum(f2 v) { const float2 t = f2_get(v); return t.x + t.y; }
 
-// Copies of 4, 8 or 16 bytes into shared memory that the thread does not wait for; `n` of them are read, the rest becomes zero.
+// Copies of 4, 8 or 16 bytes into shared memory that the thread does not wait for; with a size, so many are read and the rest is zero.
 template <int BYTES>
-__device__ __forceinline__ void copy_async(uint32_t to, const void* from, int n = BYTES) {
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from) {
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
+}
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from, int n) {
   if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(n) : "memory");
   else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(BYTES), "r"(n) : "memory");
 }
@@ -383,9 +388,14 @@ __global__ void __launch_bounds__(LN_FWD_THREADS) ln_fwd_kernel(const LnArgs a, 
 #pragma unroll
       for (int i = 0; i < V; ++i)
         if (t + i * T < npack) {
-          const int n = ln_edge<P, ODD>(t + i * T, shift, N).hi * K::ESZ;
-          copy_async<16>(ring + in + i * pitch, x_from + i * T * 16, n);
-          if constexpr (GATE) copy_async<16>(ring + in + (V + i) * pitch, g_from + i * T * 16, n);
+          if constexpr (ODD) {
+            const int n = ln_edge<P, ODD>(t + i * T, shift, N).hi * K::ESZ;
+            copy_async<16>(ring + in + i * pitch, x_from + i * T * 16, n);
+            if constexpr (GATE) copy_async<16>(ring + in + (V + i) * pitch, g_from + i * T * 16, n);
+          } else {
+            copy_async<16>(ring + in + i * pitch, x_from + i * T * 16);
+            if constexpr (GATE) copy_async<16>(ring + in + (V + i) * pitch, g_from + i * T * 16);
+          }
         }
     }
     copies_commit();
@@ -549,13 +559,13 @@ struct LnBwdPlan { int T, stages; };
 template <int DT, int V, bool ODD, bool SAVED>
 struct LnRows {
   using K = LnPack<DT>;
-  static constexpr int P = K::P, PACK = SAVED ? P : 16, UNIT = PACK / P, PLACE = LN_BWD_THREADS * PACK, BYTES = V * PLACE;
-  const char *p, *base;
+  static constexpr int P = K::P, H = K::H, PACK = SAVED ? P : 16, UNIT = PACK / P, PLACE = LN_BWD_THREADS * PACK, BYTES = V * PLACE;
+  const char *p, *base;   // the thread's first pack of the row to start; somewhere in the tensor
   long long step;
-  const uint8_t* e_from;  // the exponents of the row
+  const uint8_t* e_from;  // the exponents of the row after the one at hand, those of the thread's first pack (ODD: of the row)
   long long e_step;
   uint32_t at;
-  uint8_t e[SAVED ? V : 1], e2[SAVED && ODD ? V : 1];  // of a pack's group, and of the next one where the pack reaches into that
+  uint32_t e[SAVED ? V : 1], e2[SAVED && ODD ? V : 1];  // of a pack's group, and of the next one where the pack reaches into that
 
   __device__ void init(const void* tensor, long long ld, const int8_t* codes, const uint8_t* scales, int N, long long row, long long rows, int t, int shift, uint32_t ring) {
     base = SAVED ? reinterpret_cast<const char*>(codes) : static_cast<const char*>(tensor);
@@ -565,8 +575,13 @@ struct LnRows {
     at = ring + threadIdx.x * PACK;
     if constexpr (SAVED) {
       const int ng = (N - 1) / PK_GROUP + 1;
-      e_from = scales + row * ng;
+      e_from = scales + row * ng + (ODD ? 0 : t / K::LANES);
       e_step = rows * ng;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        e[i] = 7;
+        if constexpr (ODD) e2[i] = 7;
+      }
     }
   }
   // Zeros in the thread's places of a stage: packs behind the row's end are not copied.
@@ -582,13 +597,20 @@ struct LnRows {
 #pragma unroll
     for (int i = 0; i < V; ++i)
       if (t + i * T < npack) {
-        const int n = ln_edge<P, ODD>(t + i * T, shift, N).hi * UNIT;
-        const char* from = FILL && !live ? base : p + i * T * PACK;
-        if (ODD && SAVED && n < PACK && live) {  // part of a pack of codes: whole words, and the last one's bytes
-#pragma unroll
-          for (int w = 0; w < PACK; w += 4) copy_async<4>(stage + at + i * PLACE + w, from + (w < n ? w : 0), w < n ? min(4, n - w) : 0);
+        const char* from = p + i * T * PACK;
+        const uint32_t to = stage + at + i * PLACE;
+        if constexpr (!ODD && !FILL) {
+          copy_async<PACK>(to, from);
         } else {
-          copy_async<PACK>(stage + at + i * PLACE, from, FILL && !live ? 0 : n);
+          const int n = ln_edge<P, ODD>(t + i * T, shift, N).hi * UNIT;
+          if (FILL && !live) {
+            copy_async<PACK>(to, base, 0);
+          } else if (ODD && SAVED && n < PACK) {  // part of a pack of codes: whole words, and the last one's bytes
+#pragma unroll
+            for (int w = 0; w < PACK; w += 4) copy_async<4>(to + w, from + (w < n ? w : 0), w < n ? min(4, n - w) : 0);
+          } else {
+            copy_async<PACK>(to, from, n);
+          }
         }
       }
     p += step;
@@ -598,43 +620,46 @@ struct LnRows {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const int k = t + i * T;
-        const bool on = live && k < npack;
-        e[i] = on ? __ldg(e_from + (ODD ? max(k * P - shift, 0) / PK_GROUP : k / K::LANES)) : 7;
-        if constexpr (ODD) e2[i] = on ? __ldg(e_from + min(k * P - shift + P - 1, N - 1) / PK_GROUP) : 7;
+        if (live && k < npack) {
+          e[i] = __ldg(e_from + (ODD ? max(k * P - shift, 0) / PK_GROUP : i * T / K::LANES));
+          if constexpr (ODD) e2[i] = __ldg(e_from + min(k * P - shift + P - 1, N - 1) / PK_GROUP);
+        }
       }
       e_from += e_step;
     }
   }
-  // The values, with AFFINE times `by` plus `plus` (a checkpoint's step takes the factor in for nothing).
+  struct Words { uint32_t w[PACK / 4]; };
+  __device__ Words fetch(uint32_t stage, int i) const {
+    const uint32_t from = stage + at + i * PLACE;
+    Words v;
+    if constexpr (PACK == 16) asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]) : "r"(from) : "memory");
+    else if constexpr (PACK == 8) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.w[0]), "=r"(v.w[1]) : "r"(from) : "memory");
+    else asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v.w[0]) : "r"(from) : "memory");
+    return v;
+  }
+  // The values of pack i, with AFFINE times `by` plus `plus` (a checkpoint's step takes the factor in for nothing).
   template <bool AFFINE>
-  __device__ void get(uint32_t stage, const uint8_t* ex, const uint8_t* ex2, int t, int T, int shift, float by, float plus, f2 (*out)[K::H]) const {
+  __device__ void values(const Words& v, int i, int t, int T, int shift, float by, float plus, f2* out) const {
     const f2 plus2 = f2_all(plus);
+    if constexpr (!SAVED) {
+      K::unpack(make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]), out);
+      if constexpr (AFFINE) {
+        const f2 by2 = f2_all(by);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const uint32_t from = stage + at + i * PLACE;
-      if constexpr (!SAVED) {
-        K::unpack(shared16(from), out[i]);
-        if constexpr (AFFINE) {
-          const f2 by2 = f2_all(by);
+        for (int j = 0; j < H; ++j) out[j] = f2_fma(out[j], by2, plus2);
+      }
+    } else {
+      const float unit = AFFINE ? pk_step(e[i]) * by : pk_step(e[i]);
+      f2 units = f2_all(unit);
 #pragma unroll
-          for (int j = 0; j < K::H; ++j) out[i][j] = f2_fma(out[i][j], by2, plus2);
+      for (int c = 0; c < P; c += 2) {
+        if constexpr (ODD) {
+          // the next group begins with the value whose column is a multiple of 32
+          const float unit2 = AFFINE ? pk_step(e2[i]) * by : pk_step(e2[i]);
+          const int next = PK_GROUP - ((t + i * T) * P - shift + PK_GROUP) % PK_GROUP;
+          units = f2_of(c < next ? unit : unit2, c + 1 < next ? unit : unit2);
         }
-      } else {
-        uint32_t w[P / 4];
-        if constexpr (P == 8) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(from) : "memory");
-        else asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(from) : "memory");
-        const float unit = AFFINE ? pk_step(ex[i]) * by : pk_step(ex[i]);
-        f2 units = f2_all(unit);
-#pragma unroll
-        for (int c = 0; c < P; c += 2) {
-          if constexpr (ODD) {
-            // the next group begins with the value whose column is a multiple of 32
-            const float unit2 = AFFINE ? pk_step(ex2[i]) * by : pk_step(ex2[i]);
-            const int next = PK_GROUP - ((t + i * T) * P - shift + PK_GROUP) % PK_GROUP;
-            units = f2_of(c < next ? unit : unit2, c + 1 < next ? unit : unit2);
-          }
-          out[i][c / 2] = AFFINE ? f2_fma(pk_two(w[c / 4], c % 4), units, plus2) : f2_mul(pk_two(w[c / 4], c % 4), units);
-        }
+        out[c / 2] = AFFINE ? f2_fma(pk_two(v.w[c / 4], c % 4), units, plus2) : f2_mul(pk_two(v.w[c / 4], c % 4), units);
       }
     }
   }
@@ -664,18 +689,18 @@ __device__ __forceinline__ float2 team_sum(float2 v, uint32_t slot, int t, int T
     } else {
       if ((t & 15) == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(slot + (t >> 4) * 4), "f"(keep) : "memory");
       asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(T) : "memory");
-      float4 s = shared_f4(slot);
-      const auto more = [&](int from, int to) {
+      f2 s = 0;
+      const auto add = [&](int from, int to) {
 #pragma unroll
         for (int w = from; w < to; ++w) {
           const float4 u = shared_f4(slot + w * 16);
-          s = make_float4(s.x + u.x, s.y + u.y, s.z + u.z, s.w + u.w);
+          s = f2_add(s, f2_add(f2_of(u.x, u.y), f2_of(u.z, u.w)));
         }
       };
-      if (T > 64) more(1, 2);
-      if (T > 128) more(2, 4);
-      if (T > 256) more(4, 8);
-      return make_float2(s.x + s.z, s.y + s.w);
+      add(0, 2);
+      if (T > 128) add(2, 4);
+      if (T > 256) add(4, 8);
+      return f2_get(s);
     }
   }
 }
@@ -684,7 +709,10 @@ template <int DT, int E, int G, bool ODD, bool GATE, bool SAVED>
 __global__ void __launch_bounds__(LN_BWD_THREADS) ln_bwd_kernel(const LnArgs a, const LnBwdPlan plan) {
   using K = LnPack<DT>;
   constexpr int P = K::P, H = K::H, V = E / P;
-  constexpr bool FILL = G < 32, PLANES = GATE && !ODD;  // weight and bias in shared memory where registers would not do
+  constexpr bool FILL = G < 32;
+  // Weight and bias: in registers, or, with a gate, where these would not do: in shared memory (PLANES), or, in fp32, where that would not
+  // either, read again for each row.
+  constexpr bool PLANES = GATE && !ODD && DT != SRMS_F32, AGAIN = GATE && !ODD && !PLANES, HELD = !PLANES && !AGAIN;
   using In = LnRows<DT, V, ODD, SAVED>;
   using Dy = LnRows<DT, V, ODD, false>;
   constexpr uint32_t STAGE = Dy::BYTES + In::BYTES * (GATE ? 2 : 1), SLOTS = G > 32 ? LN_BWD_SLOTS : 0;
@@ -692,8 +720,9 @@ __global__ void __launch_bounds__(LN_BWD_THREADS) ln_bwd_kernel(const LnArgs a, 
   const int N = a.N;
   const float inv_n = 1.f / static_cast<float>(N);
   // shared memory: the teams' slots, weight and bias, the ring
-  const uint32_t slots = static_cast<uint32_t>(__cvta_generic_to_shared(ln_shared)), wplane = slots + SLOTS, bplane = wplane + N * 4;
-  const uint32_t ring = PLANES ? bplane + N * 4 : wplane, ring_end = plan.stages * STAGE;
+  constexpr uint32_t PLANE = LN_BWD_THREADS * V * 16;  // four values of each pack
+  const uint32_t slots = static_cast<uint32_t>(__cvta_generic_to_shared(ln_shared)), planes = slots + SLOTS;
+  const uint32_t ring = PLANES ? planes + 2 * (P / 4) * PLANE : planes, ring_end = plan.stages * STAGE;
   uint32_t slot = slots + (G > 32 ? team * 256 : 0);
   if constexpr (G > 32)
     for (int i = threadIdx.x; i < SLOTS / 4; i += lanes) asm volatile("st.shared.u32 [%0], %1;" ::"r"(slots + 4 * i), "r"(0) : "memory");
@@ -719,12 +748,14 @@ __global__ void __launch_bounds__(LN_BWD_THREADS) ln_bwd_kernel(const LnArgs a, 
     in = in + STAGE == ring_end ? 0 : in + STAGE;
   };
   const float2* st_from = a.stats + row;
-  float2 st_next;
+  float2 st = make_float2(0.f, 0.f);
   const auto start_small = [&](int n) {
-    st_next = n < mine ? __ldg(st_from) : make_float2(0.f, 0.f);
+    const bool live = n < mine;
+    if (FILL && !live) st = make_float2(0.f, 0.f);
+    if (live) st = __ldg(st_from);
     st_from += step;
-    x.start_scales(n < mine, t, T, npack, shift, N);
-    if constexpr (GATE) g.start_scales(n < mine, t, T, npack, shift, N);
+    x.start_scales(live, t, T, npack, shift, N);
+    if constexpr (GATE) g.start_scales(live, t, T, npack, shift, N);
   };
   for (int k = 0; k < plan.stages; ++k) {
     dy.clear(k * STAGE);
@@ -733,119 +764,125 @@ __global__ void __launch_bounds__(LN_BWD_THREADS) ln_bwd_kernel(const LnArgs a, 
   }
   for (int k = 1; k < plan.stages; ++k) start(k - 1);
   start_small(0);
-  f2 w[PLANES ? 1 : V][H], b[GATE && !PLANES ? V : 1][H], dw[V][H], db[V][H];
+  f2 w[HELD ? V : 1][H], b[HELD && GATE ? V : 1][H], dw[V][H], db[V][H];
+  const auto columns = [&](int i, bool bias, f2* out) {  // weight or bias of pack i's columns
+    const int k = t + i * T;
+    const void* from = bias ? a.bias : a.weight;
+    if constexpr (ODD) {
+      K::params_at(from, a.wdt, k * P - shift, N, bias ? 0.f : 1.f, out);
+    } else {
+      float f[P];
+      K::params(k < npack ? from : nullptr, a.wdt, a.vec_params, k, bias ? 0.f : 1.f, f);
+#pragma unroll
+      for (int j = 0; j < H; ++j) out[j] = f2_of(f[2 * j], f[2 * j + 1]);
+    }
+  };
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int k = t + i * T;
-    if constexpr (ODD) {
-      K::params_at(a.weight, a.wdt, k * P - shift, N, 1.f, w[i]);
-      if constexpr (GATE) K::params_at(a.bias, a.wdt, k * P - shift, N, 0.f, b[i]);
-    } else if constexpr (!PLANES) {
-      float f[P];
-      K::params(k < npack ? a.weight : nullptr, a.wdt, a.vec_params, k, 1.f, f);
-#pragma unroll
-      for (int j = 0; j < H; ++j) w[i][j] = f2_of(f[2 * j], f[2 * j + 1]);
-    }
+    if constexpr (HELD) columns(i, false, w[i]);
+    if constexpr (HELD && GATE) columns(i, true, b[i]);
 #pragma unroll
     for (int j = 0; j < H; ++j) dw[i][j] = db[i][j] = 0;
   }
   if constexpr (PLANES)
-    for (int k = threadIdx.x; k < npack; k += lanes) {
-      float f[P];
-      K::params(a.weight, a.wdt, a.vec_params, k, 1.f, f);
-      K::plane_put(wplane, npack, k, f);
-      K::params(a.bias, a.wdt, a.vec_params, k, 0.f, f);
-      K::plane_put(bplane, npack, k, f);
+    for (int k = threadIdx.x; k < V * T; k += lanes)  // those behind the row's end too: they are multiplied by zero
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        float f[P];
+        K::params(k >= npack ? nullptr : which ? a.bias : a.weight, a.wdt, a.vec_params, k, which ? 0.f : 1.f, f);
+#pragma unroll
+        for (int e = 0; e < P; e += 4) shared_put(planes + (which * (P / 4) + e / 4) * PLANE + k * 16, make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]));
+      }
+  // Weight or bias of pack i from where they are.
+  const auto weights = [&](int i, bool bias, f2* out) {
+    if constexpr (PLANES) {
+#pragma unroll
+      for (int e = 0; e < P; e += 4) {
+        const float4 v = shared_f4(planes + t * 16 + i * T * 16 + ((bias ? P / 4 : 0) + e / 4) * PLANE);
+        out[e / 2] = f2_of(v.x, v.y);
+        out[e / 2 + 1] = f2_of(v.z, v.w);
+      }
+    } else if constexpr (AGAIN) {
+      columns(i, bias, out);
+    } else {
+#pragma unroll
+      for (int j = 0; j < H; ++j) out[j] = bias ? b[GATE ? i : 0][j] : w[i][j];
     }
+  };
   if constexpr (PLANES || G > 32) __syncthreads();
   char *dx = static_cast<char*>(a.dx) + (row * N - shift) * K::ESZ + t * 16, *dg = static_cast<char*>(a.dgate) + (row * N - shift) * K::ESZ + t * 16;
   const long long out_step = step * N * K::ESZ;
   for (int n = 0; n < most; ++n, dx += out_step, dg += out_step) {
     const bool live = !FILL || n < mine;
     copies_wait(plan.stages);
-    const float2 st = st_next;
-    uint8_t ex[SAVED ? V : 1], eg[SAVED && GATE ? V : 1], ex2[SAVED && ODD ? V : 1], eg2[SAVED && GATE && ODD ? V : 1];
-    if constexpr (SAVED) {
+    const float r = st.y, minus_mr = -st.x * st.y;
+    f2 xh[V][H], s[V][H];  // s: dy, then with the gate's factor, then with the weight's
+    f2 c1 = 0, c2 = 0;
+    typename Dy::Words dy_words[V];
+    typename In::Words x_words[V], g_words[GATE ? V : 1];
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        ex[i] = x.e[i];
-        if constexpr (ODD) ex2[i] = x.e2[i];
-        if constexpr (GATE) eg[i] = g.e[i];
-        if constexpr (GATE && ODD) eg2[i] = g.e2[i];
+    for (int i = 0; i < V; ++i) {
+      dy_words[i] = dy.fetch(out, i);
+      x_words[i] = x.fetch(out, i);
+      if constexpr (GATE) g_words[i] = g.fetch(out, i);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const LnPackEdge e = ln_edge<P, ODD>(t + i * T, shift, N);
+      dy.template values<false>(dy_words[i], i, t, T, shift, 1.f, 0.f, s[i]);
+      x.template values<true>(x_words[i], i, t, T, shift, r, minus_mr, xh[i]);
+      if (ODD && (e.lo > 0 || e.hi < P)) {
+        K::cut(s[i], e.lo, e.hi);
+        K::cut(xh[i], e.lo, e.hi);
       }
     }
-    f2 xh[V][H], s[V][H];
-    dy.template get<false>(out, nullptr, nullptr, t, T, shift, 1.f, 0.f, s);
-    x.template get<true>(out, ex, ex2, t, T, shift, st.y, -st.x * st.y, xh);
-    if constexpr (ODD) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const LnPackEdge e = ln_edge<P, ODD>(t + i * T, shift, N);
-        if (e.lo > 0 || e.hi < P) {
-          K::cut(s[i], e.lo, e.hi);
-          K::cut(xh[i], e.lo, e.hi);
-        }
-      }
-    }
-    const f2 rr = f2_all(st.y);
     if constexpr (GATE) {
-      f2 u[V][H];
-      g.template get<true>(out, eg, eg2, t, T, shift, LN_MINUS_LOG2E, 0.f, u);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const int k = t + i * T;
+        const LnPackEdge e = ln_edge<P, ODD>(k, shift, N);
+        const bool part = ODD && (e.lo > 0 || e.hi < P);
         if (k < npack) {
-          f2 wk[H], bk[H];
-          if constexpr (PLANES) {
-            K::plane_get(wplane, npack, k, wk);
-            K::plane_get(bplane, npack, k, bk);
-          } else {
-#pragma unroll
-            for (int j = 0; j < H; ++j) { wk[j] = w[i][j]; bk[j] = b[i][j]; }
-          }
-          const LnPackEdge e = ln_edge<P, ODD>(k, shift, N);
-          if (ODD && (e.lo > 0 || e.hi < P)) K::cut(u[i], e.lo, e.hi);
+          f2 u[H], wk[H], bk[H];
+          g.template values<true>(g_words[i], i, t, T, shift, LN_MINUS_LOG2E, 0.f, u);
+          if (part) K::cut(u, e.lo, e.hi);
+          weights(i, false, wk);
+          weights(i, true, bk);
 #pragma unroll
           for (int j = 0; j < H; ++j) {
-            const float2 gv = f2_get(u[i][j]);
+            const float2 gv = f2_get(u[j]);
             float s0, s1, r0, r1;
             ln_sigmoid2(gv.x, &s0, &r0);
             ln_sigmoid2(gv.y, &s1, &r1);
             s[i][j] = f2_mul(s[i][j], f2_of(s0, s1));
-            u[i][j] = f2_mul(f2_mul(s[i][j], f2_fma(xh[i][j], wk[j], bk[j])), f2_of(r0, r1));
+            u[j] = f2_mul(f2_mul(s[i][j], f2_fma(xh[i][j], wk[j], bk[j])), f2_of(r0, r1));
           }
           if (a.dgate && live) {
-            if (ODD && (e.lo > 0 || e.hi < P)) K::store_part(dg + i * T * 16, u[i], e.lo, e.hi);
-            else K::store(dg + i * T * 16, u[i]);
+            if (part) K::store_part(dg + i * T * 16, u, e.lo, e.hi);
+            else K::store(dg + i * T * 16, u);
           }
         }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      f2 wk[H];
+      weights(i, false, wk);
+#pragma unroll
+      for (int j = 0; j < H; ++j) {
+        db[i][j] = f2_add(db[i][j], s[i][j]);
+        dw[i][j] = f2_fma(s[i][j], xh[i][j], dw[i][j]);
+        s[i][j] = f2_mul(wk[j], s[i][j]);
+        c1 = f2_add(c1, s[i][j]);
+        c2 = f2_fma(s[i][j], xh[i][j], c2);
       }
     }
     out = out + STAGE == ring_end ? 0 : out + STAGE;
     start(n + plan.stages - 1);
     start_small(n + 1);
-    f2 c1 = 0, c2 = 0;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      f2 wk[H];
-      if constexpr (PLANES) {
-#pragma unroll
-        for (int j = 0; j < H; ++j) wk[j] = 0;
-        if (t + i * T < npack) K::plane_get(wplane, npack, t + i * T, wk);
-      }
-#pragma unroll
-      for (int j = 0; j < H; ++j) {
-        const f2 wij = PLANES ? wk[j] : w[PLANES ? 0 : i][j];
-        db[i][j] = f2_add(db[i][j], s[i][j]);
-        const f2 p = f2_mul(s[i][j], xh[i][j]);
-        dw[i][j] = f2_add(dw[i][j], p);
-        c2 = f2_fma(wij, p, c2);
-        s[i][j] = f2_mul(wij, s[i][j]);
-        c1 = f2_add(c1, s[i][j]);
-      }
-    }
     const float2 c = team_sum<G>(make_float2(f2_sum(c1), f2_sum(c2)), slot, t, T, team);
-    const f2 k1 = f2_all(-c.x * inv_n * st.y), k2 = f2_all(-c.y * inv_n * st.y);
+    const float by = -inv_n * r;
+    const f2 rr = f2_all(r), k1 = f2_all(c.x * by), k2 = f2_all(c.y * by);
     if (a.dx && live) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
