@@ -362,49 +362,65 @@ extern __shared__ __align__(16) char ln_shared[];
 // A row is a team's of T threads, V packs a thread: T a power of two up to 32 (several rows in a warp) or a multiple of 32. A warp
 // has the mean and the squares about it of its part of a row from shuffles; the parts are joined by the formula for the variance of
 // a union, behind the only barrier of a row. Each thread has places of its own in the ring of copies, so that it needs none.
-constexpr int LN_FWD_THREADS = 640;  // most of a CTA: 20 warps of up to 96 registers hide more than 16 do (32768 x 4096: 95 us, 106)
+// Most threads of a CTA: 20 warps of up to 96 registers hide more than 16 of 128 do (32768 x 4096 bf16: 95 us, 106), but for the gated
+// norm that writes checkpoints, which spills then.
+template <bool GATE, bool SAVE> constexpr int LN_FWD_THREADS = GATE && SAVE ? 512 : 640;
 
-struct LnFwdPlan { int T, stages; };
+// Strides from one of a team's rows to its next, in bytes: all teams' rows at once. As arguments they cost the kernels no registers.
+struct LnSteps {
+  long long rows, x, gate, dy, out, codes, scales;
+  LnSteps() = default;
+  LnSteps(const LnArgs& a, int esz, long long all_teams)
+      : rows(all_teams), x(all_teams * a.ldx * esz), gate(all_teams * a.ldg * esz), dy(all_teams * a.lddy * esz), out(all_teams * a.N * esz),
+        codes(all_teams * a.N), scales(all_teams * ((a.N - 1) / PK_GROUP + 1)) {}
+};
+
+struct LnFwdPlan { int T, stages; LnSteps step; };
 
 template <int DT, int V, int G, bool ODD, bool GATE, bool SAVE>
-__global__ void __launch_bounds__(LN_FWD_THREADS) ln_fwd_kernel(const LnArgs a, const LnFwdPlan plan) {
+__global__ void __launch_bounds__((LN_FWD_THREADS<GATE, SAVE>)) ln_fwd_kernel(const LnArgs a, const LnFwdPlan plan) {
   using K = LnPack<DT>;
   constexpr int P = K::P, H = K::H;
   static_assert(!(ODD && SAVE), "groups of 32 values do not keep to the packs of odd rows");
-  __shared__ float4 slot[G > 32 ? 2 : 1][LN_FWD_THREADS / 32];  // of a CTA's warps: mean, squares, count of their part; two halves in turn
-  const int T = G <= 32 ? G : plan.T, team = threadIdx.x / T, t = threadIdx.x - team * T, lanes = blockDim.x, warp = threadIdx.x >> 5;
+  // of each team's warps: mean, squares, count of their part; two halves in turn. What a team does not fill has a count of zero.
+  constexpr int THREADS = (LN_FWD_THREADS<GATE, SAVE>), WARPS = THREADS / 32, TEAMS = G > 32 ? THREADS / 64 : 1;
+  __shared__ float4 slots[TEAMS][2][WARPS];
+  const int T = G <= 32 ? G : plan.T, team = threadIdx.x / T, t = threadIdx.x - team * T, lanes = blockDim.x, warp = t >> 5;
   const int N = a.N, ng = (N - 1) / PK_GROUP + 1, teams = lanes / T;
   const uint32_t wplane = static_cast<uint32_t>(__cvta_generic_to_shared(ln_shared)), bplane = wplane + N * 4, ring = (ODD ? wplane : bplane + N * 4) + threadIdx.x * 16;
-  const uint32_t pitch = lanes * 16, stage_bytes = pitch * V * (GATE ? 2 : 1), ring_end = plan.stages * stage_bytes;
-  const long long step = static_cast<long long>(gridDim.x) * teams;
-  long long row = static_cast<long long>(blockIdx.x) * teams + team, ahead = row;
-  long long first = G < 32 ? static_cast<long long>(blockIdx.x) * teams + (threadIdx.x & ~31) / T : row;
+  constexpr uint32_t PITCH = THREADS * 16, STAGE = PITCH * V * (GATE ? 2 : 1);
+  const uint32_t ring_end = plan.stages * STAGE;
+  if constexpr (G > 32)
+    for (int i = threadIdx.x; i < TEAMS * 2 * WARPS; i += lanes) slots[0][0][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  const long long row = static_cast<long long>(blockIdx.x) * teams + team;
+  const long long first = G < 32 ? static_cast<long long>(blockIdx.x) * teams + (threadIdx.x & ~31) / T : row;
+  // rows of this team, and of the team in its warp that has most
+  const int mine = row < a.M ? static_cast<int>((a.M - 1 - row) / plan.step.rows) + 1 : 0;
+  const int most = G >= 32 ? mine : first < a.M ? static_cast<int>((a.M - 1 - first) / plan.step.rows) + 1 : 0;
   const int shift = ODD ? static_cast<int>(row * N % P) : 0, npack = (N + shift + P - 1) / P;
   const char *x_from = static_cast<const char*>(a.x) + (row * a.ldx - shift) * K::ESZ + t * 16, *g_from = static_cast<const char*>(a.gate) + (row * a.ldg - shift) * K::ESZ + t * 16;
-  const long long x_step = step * a.ldx * K::ESZ, g_step = step * a.ldg * K::ESZ;
   uint32_t in = 0, out = 0;
-  const auto start = [&] {
-    if (ahead < a.M) {
+  const auto start = [&](int n) {
+    if (n < mine) {
 #pragma unroll
       for (int i = 0; i < V; ++i)
         if (t + i * T < npack) {
           if constexpr (ODD) {
-            const int n = ln_edge<P, ODD>(t + i * T, shift, N).hi * K::ESZ;
-            copy_async<16>(ring + in + i * pitch, x_from + i * T * 16, n);
-            if constexpr (GATE) copy_async<16>(ring + in + (V + i) * pitch, g_from + i * T * 16, n);
+            const int size = ln_edge<P, ODD>(t + i * T, shift, N).hi * K::ESZ;
+            copy_async<16>(ring + in + i * PITCH, x_from + i * T * 16, size);
+            if constexpr (GATE) copy_async<16>(ring + in + (V + i) * PITCH, g_from + i * T * 16, size);
           } else {
-            copy_async<16>(ring + in + i * pitch, x_from + i * T * 16);
-            if constexpr (GATE) copy_async<16>(ring + in + (V + i) * pitch, g_from + i * T * 16);
+            copy_async<16>(ring + in + i * PITCH, x_from + i * T * 16);
+            if constexpr (GATE) copy_async<16>(ring + in + (V + i) * PITCH, g_from + i * T * 16);
           }
         }
     }
     copies_commit();
-    ahead += step;
-    x_from += x_step;
-    g_from += g_step;
-    in = in + stage_bytes == ring_end ? 0 : in + stage_bytes;
+    x_from += plan.step.x;
+    if constexpr (GATE) g_from += plan.step.gate;
+    in = in + STAGE == ring_end ? 0 : in + STAGE;
   };
-  for (int k = 1; k < plan.stages; ++k) start();
+  for (int k = 1; k < plan.stages; ++k) start(k - 1);
   // weight and bias: in shared memory, or, where each team has columns of its own in a pack, in registers
   f2 wr[ODD ? V : 1][H], br[ODD ? V : 1][H];
   if constexpr (ODD) {
@@ -421,8 +437,8 @@ __global__ void __launch_bounds__(LN_FWD_THREADS) ln_fwd_kernel(const LnArgs a, 
       K::params(a.bias, a.wdt, a.vec_params, k, 0.f, f);
       K::plane_put(bplane, npack, k, f);
     }
-    __syncthreads();
   }
+  if constexpr (!ODD || G > 32) __syncthreads();
   int count = 0;  // values of a row that this warp (or sub-warp team) has
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -434,16 +450,19 @@ __global__ void __launch_bounds__(LN_FWD_THREADS) ln_fwd_kernel(const LnArgs a, 
   const float fcount = static_cast<float>(count), inv_count = count ? 1.f / fcount : 0.f, inv_n = 1.f / static_cast<float>(N);
   int turn = 0;
   char* y = static_cast<char*>(a.y) + (row * N - shift) * K::ESZ + t * 16;
-  const long long y_step = step * N * K::ESZ;
-  for (; first < a.M; first += step, row += step, y += y_step) {
-    const bool live = G >= 32 || row < a.M;
+  int8_t* xc = SAVE ? a.xcodes + row * N : nullptr;
+  uint8_t* xs = SAVE ? a.xscales + row * ng : nullptr;
+  const long long gate_codes = a.gcodes - a.xcodes, gate_scales = a.gscales - a.xscales;  // from x's to the gate's
+  float2* stats = a.stats ? a.stats + row : nullptr;
+  for (int n = 0; n < most; ++n, y += plan.step.out) {
+    const bool live = G >= 32 || n < mine;
     copies_wait(plan.stages);
     uint4 raw[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) raw[i] = live && t + i * T < npack ? shared16(ring + out + i * pitch) : make_uint4(0, 0, 0, 0);
-    const uint32_t gates = ring + out + V * pitch;
-    out = out + stage_bytes == ring_end ? 0 : out + stage_bytes;
-    start();
+    for (int i = 0; i < V; ++i) raw[i] = live && t + i * T < npack ? shared16(ring + out + i * PITCH) : make_uint4(0, 0, 0, 0);
+    const uint32_t gates = ring + out + V * PITCH;
+    out = out + STAGE == ring_end ? 0 : out + STAGE;
+    start(n + plan.stages - 1);
     f2 v[V][H];
     f2 s = 0;
 #pragma unroll
@@ -455,7 +474,7 @@ __global__ void __launch_bounds__(LN_FWD_THREADS) ln_fwd_kernel(const LnArgs a, 
 #pragma unroll
       for (int j = 1; j < H; ++j) part = f2_add(part, v[i][j]);
       s = f2_add(s, part);
-      if constexpr (SAVE) K::quantise(raw[i], v[i], a.xcodes + row * N, a.xscales + row * ng, t + i * T, live && t + i * T < npack);
+      if constexpr (SAVE) K::quantise(raw[i], v[i], xc, xs, t + i * T, live && t + i * T < npack);
     }
     float m = f2_sum(s);
 #pragma unroll
@@ -490,22 +509,29 @@ __global__ void __launch_bounds__(LN_FWD_THREADS) ln_fwd_kernel(const LnArgs a, 
     float mean = q1 * inv_count;  // counted from m
     float squares = fmaf(-mean, q1, q2);
     if constexpr (G > 32) {
-      if ((t & 31) == 0) slot[turn][warp] = make_float4(m + mean, squares, fcount, 0.f);
+      float4* slot = slots[team][turn];
+      if ((t & 31) == 0) slot[warp] = make_float4(m + mean, squares, fcount, 0.f);
       asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(T) : "memory");
-      const float4* part = slot[turn] + team * (T / 32);
       float total = 0.f, both = 0.f;
-      for (int w = 0; w < T / 32; ++w) {
-        const float d = part[w].x - m;
-        total = fmaf(part[w].z, d, total);
-        both += fmaf(part[w].z * d, d, part[w].y);
-      }
+      const auto join = [&](int from, int to) {
+#pragma unroll
+        for (int w = from; w < to; ++w) {
+          const float d = slot[w].x - m, zd = slot[w].z * d;
+          total += zd;
+          both += fmaf(zd, d, slot[w].y);
+        }
+      };
+      join(0, 4);
+      if (T > 128) join(4, 8);
+      if (T > 256) join(8, WARPS);
       mean = total * inv_n;
       squares = fmaf(-mean, total, both);
       turn ^= 1;
     }
     squares *= inv_n;
     const float r = 1.f / sqrtf((squares < 0.f ? 0.f : squares) + a.eps);
-    if (a.stats && t == 0 && live) a.stats[row] = make_float2(m + mean, r);
+    if (stats && t == 0 && live) *stats = make_float2(m + mean, r);
+    if (a.stats) stats += plan.step.rows;
     const f2 off = f2_all(-mean * r), rr = f2_all(r);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -513,9 +539,9 @@ __global__ void __launch_bounds__(LN_FWD_THREADS) ln_fwd_kernel(const LnArgs a, 
       const bool on = live && k < npack;
       f2 u[H];
       if constexpr (GATE) {
-        const uint4 words = on ? shared16(gates + i * pitch) : make_uint4(0, 0, 0, 0);
+        const uint4 words = on ? shared16(gates + i * PITCH) : make_uint4(0, 0, 0, 0);
         K::unpack(words, u);
-        if constexpr (SAVE) K::quantise(words, u, a.gcodes + row * N, a.gscales + row * ng, k, on);
+        if constexpr (SAVE) K::quantise(words, u, xc + gate_codes, xs + gate_scales, k, on);
 #pragma unroll
         for (int j = 0; j < H; ++j) u[j] = f2_mul(u[j], f2_all(LN_MINUS_LOG2E));
       }
@@ -541,6 +567,10 @@ __global__ void __launch_bounds__(LN_FWD_THREADS) ln_fwd_kernel(const LnArgs a, 
         else K::store(y + i * T * 16, v[i]);
       }
     }
+    if constexpr (SAVE) {
+      xc += plan.step.codes;
+      xs += plan.step.scales;
+    }
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
@@ -552,7 +582,7 @@ __global__ void __launch_bounds__(LN_FWD_THREADS) ln_fwd_kernel(const LnArgs a, 
 constexpr int LN_BWD_THREADS = 512;  // most of a CTA
 constexpr int LN_BWD_SLOTS = LN_BWD_THREADS / 64 * 2 * 128;  // two halves of 16 warps' two sums for each team of several warps
 
-struct LnBwdPlan { int T, stages; };
+struct LnBwdPlan { int T, stages; LnSteps step; };
 
 // What a team reads row by row: a tensor, or (SAVED) its checkpoint.
 // PLACE: bytes from a thread's place for one pack to that for the next.
@@ -561,22 +591,18 @@ struct LnRows {
   using K = LnPack<DT>;
   static constexpr int P = K::P, H = K::H, PACK = SAVED ? P : 16, UNIT = PACK / P, PLACE = LN_BWD_THREADS * PACK, BYTES = V * PLACE;
   const char *p, *base;   // the thread's first pack of the row to start; somewhere in the tensor
-  long long step;
   const uint8_t* e_from;  // the exponents of the row after the one at hand, those of the thread's first pack (ODD: of the row)
-  long long e_step;
   uint32_t at;
   uint32_t e[SAVED ? V : 1], e2[SAVED && ODD ? V : 1];  // of a pack's group, and of the next one where the pack reaches into that
 
-  __device__ void init(const void* tensor, long long ld, const int8_t* codes, const uint8_t* scales, int N, long long row, long long rows, int t, int shift, uint32_t ring) {
+  __device__ void init(const void* tensor, long long ld, const int8_t* codes, const uint8_t* scales, int N, long long row, int t, int shift, uint32_t ring) {
     base = SAVED ? reinterpret_cast<const char*>(codes) : static_cast<const char*>(tensor);
     const long long pitch = SAVED ? N : ld;
     p = base + (row * pitch - shift) * UNIT + t * PACK;
-    step = rows * pitch * UNIT;
     at = ring + threadIdx.x * PACK;
     if constexpr (SAVED) {
       const int ng = (N - 1) / PK_GROUP + 1;
       e_from = scales + row * ng + (ODD ? 0 : t / K::LANES);
-      e_step = rows * ng;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         e[i] = 7;
@@ -593,7 +619,7 @@ struct LnRows {
   }
   // FILL: teams that share a warp, of which one may have no row: its places become zero.
   template <bool FILL>
-  __device__ void start(uint32_t stage, bool live, int t, int T, int npack, int shift, int N) {
+  __device__ void start(uint32_t stage, bool live, int t, int T, int npack, int shift, int N, long long step) {
 #pragma unroll
     for (int i = 0; i < V; ++i)
       if (t + i * T < npack) {
@@ -615,7 +641,7 @@ struct LnRows {
       }
     p += step;
   }
-  __device__ void start_scales(bool live, int t, int T, int npack, int shift, int N) {
+  __device__ void start_scales(bool live, int t, int T, int npack, int shift, int N, long long step) {
     if constexpr (SAVED) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
@@ -625,7 +651,7 @@ struct LnRows {
           if constexpr (ODD) e2[i] = __ldg(e_from + min(k * P - shift + P - 1, N - 1) / PK_GROUP);
         }
       }
-      e_from += e_step;
+      e_from += step;
     }
   }
   struct Words { uint32_t w[PACK / 4]; };
@@ -726,23 +752,23 @@ __global__ void __launch_bounds__(LN_BWD_THREADS) ln_bwd_kernel(const LnArgs a, 
   uint32_t slot = slots + (G > 32 ? team * 256 : 0);
   if constexpr (G > 32)
     for (int i = threadIdx.x; i < SLOTS / 4; i += lanes) asm volatile("st.shared.u32 [%0], %1;" ::"r"(slots + 4 * i), "r"(0) : "memory");
-  const long long step = static_cast<long long>(gridDim.x) * teams;
   const long long row = static_cast<long long>(blockIdx.x) * teams + team;
   const long long first = FILL ? static_cast<long long>(blockIdx.x) * teams + (threadIdx.x & ~31) / T : row;
   // rows of this team, and of the team in its warp that has most
-  const int mine = row < a.M ? static_cast<int>((a.M - 1 - row) / step) + 1 : 0, most = first < a.M ? static_cast<int>((a.M - 1 - first) / step) + 1 : 0;
+  const int mine = row < a.M ? static_cast<int>((a.M - 1 - row) / plan.step.rows) + 1 : 0;
+  const int most = !FILL ? mine : first < a.M ? static_cast<int>((a.M - 1 - first) / plan.step.rows) + 1 : 0;
   const int shift = ODD ? static_cast<int>(row * N % P) : 0, npack = (N + shift + P - 1) / P;
   In x, g;
   Dy dy;
-  dy.init(a.dy, a.lddy, nullptr, nullptr, N, row, step, t, shift, ring);
-  x.init(a.x, a.ldx, a.xcodes, a.xscales, N, row, step, t, shift, ring + Dy::BYTES);
-  if constexpr (GATE) g.init(a.gate, a.ldg, a.gcodes, a.gscales, N, row, step, t, shift, ring + Dy::BYTES + In::BYTES);
+  dy.init(a.dy, a.lddy, nullptr, nullptr, N, row, t, shift, ring);
+  x.init(a.x, a.ldx, a.xcodes, a.xscales, N, row, t, shift, ring + Dy::BYTES);
+  if constexpr (GATE) g.init(a.gate, a.ldg, a.gcodes, a.gscales, N, row, t, shift, ring + Dy::BYTES + In::BYTES);
   uint32_t in = 0, out = 0;
   const auto start = [&](int n) {
     if (FILL || n < mine) {
-      dy.template start<FILL>(in, n < mine, t, T, npack, shift, N);
-      x.template start<FILL>(in, n < mine, t, T, npack, shift, N);
-      if constexpr (GATE) g.template start<FILL>(in, n < mine, t, T, npack, shift, N);
+      dy.template start<FILL>(in, n < mine, t, T, npack, shift, N, plan.step.dy);
+      x.template start<FILL>(in, n < mine, t, T, npack, shift, N, SAVED ? plan.step.codes : plan.step.x);
+      if constexpr (GATE) g.template start<FILL>(in, n < mine, t, T, npack, shift, N, SAVED ? plan.step.codes : plan.step.gate);
     }
     copies_commit();
     in = in + STAGE == ring_end ? 0 : in + STAGE;
@@ -753,9 +779,9 @@ __global__ void __launch_bounds__(LN_BWD_THREADS) ln_bwd_kernel(const LnArgs a, 
     const bool live = n < mine;
     if (FILL && !live) st = make_float2(0.f, 0.f);
     if (live) st = __ldg(st_from);
-    st_from += step;
-    x.start_scales(live, t, T, npack, shift, N);
-    if constexpr (GATE) g.start_scales(live, t, T, npack, shift, N);
+    st_from += plan.step.rows;
+    x.start_scales(live, t, T, npack, shift, N, plan.step.scales);
+    if constexpr (GATE) g.start_scales(live, t, T, npack, shift, N, plan.step.scales);
   };
   for (int k = 0; k < plan.stages; ++k) {
     dy.clear(k * STAGE);
@@ -811,8 +837,7 @@ __global__ void __launch_bounds__(LN_BWD_THREADS) ln_bwd_kernel(const LnArgs a, 
   };
   if constexpr (PLANES || G > 32) __syncthreads();
   char *dx = static_cast<char*>(a.dx) + (row * N - shift) * K::ESZ + t * 16, *dg = static_cast<char*>(a.dgate) + (row * N - shift) * K::ESZ + t * 16;
-  const long long out_step = step * N * K::ESZ;
-  for (int n = 0; n < most; ++n, dx += out_step, dg += out_step) {
+  for (int n = 0; n < most; ++n, dx += plan.step.out, dg += plan.step.out) {
     const bool live = !FILL || n < mine;
     copies_wait(plan.stages);
     const float r = st.y, minus_mr = -st.x * st.y;

@@ -63,14 +63,16 @@ cudaError_t ln_fwd_any(const LnArgs& a, LnPlace at) {
 template <int DT, int V, int G, bool ODD>
 cudaError_t ln_fwd_team(const LnArgs& a, LnPlace at, int T) {
   const bool gate = a.gate, save = a.xcodes;
-  const int teams = LN_FWD_THREADS / T, cta = teams * T, stage = cta * 16 * V * (gate ? 2 : 1);
+  const int threads = gate && save ? LN_FWD_THREADS<true, true> : LN_FWD_THREADS<false, false>, teams = threads / T, cta = teams * T, stage = threads * 16 * V * (gate ? 2 : 1);
   const size_t planes = ODD ? 0 : static_cast<size_t>(a.N) * 8;
-  int stages = planes > LN_SHARED - 2048 ? 0 : static_cast<int>((LN_SHARED - 2048 - planes) / stage);
+  // beside the kernel's slots
+  constexpr size_t room = LN_SHARED - (G > 32 ? 640 / 64 * 2 * (640 / 32) * 16 : 640);
+  int stages = planes > room ? 0 : static_cast<int>((room - planes) / stage);
   if (stages < 2) return ln_fwd_any<DT>(a, at);
   stages = stages > 4 ? 4 : stages;
-  const LnFwdPlan plan{T, stages};
   const size_t shared = planes + static_cast<size_t>(stages) * stage;
   const unsigned grid = static_cast<unsigned>(ln_even((a.M + teams - 1) / teams, at.sms, teams, ODD ? ln_period(a.N, LnPack<DT>::P) : 1));
+  const LnFwdPlan plan{T, stages, LnSteps(a, LnPack<DT>::ESZ, static_cast<long long>(grid) * teams)};
   if constexpr (ODD) {
     return gate ? ln_launch(ln_fwd_kernel<DT, V, G, true, true, false>, grid, cta, shared, at.st, a, plan)
                 : ln_launch(ln_fwd_kernel<DT, V, G, true, false, false>, grid, cta, shared, at.st, a, plan);
@@ -129,11 +131,13 @@ bool ln_bwd_plan(const LnArgs& a, LnPlace at, LnBwdLaunch* l) {
   const size_t sums = odd ? static_cast<size_t>(a.N) * 4 : static_cast<size_t>(units - 1) * E * T * 4;
   const int stages = fixed > LN_SHARED ? 0 : static_cast<int>((LN_SHARED - fixed) / stage);
   if (stages < 2) return false;
-  l->plan = {T, stages > 4 ? 4 : stages};
+  l->plan.T = T;
+  l->plan.stages = stages > 4 ? 4 : stages;
   l->shared = fixed + l->plan.stages * stage;
   if (sums > l->shared) l->shared = sums;
   const long long most = at.sms < LN_MAX_PARTS ? at.sms : LN_MAX_PARTS;
   l->parts = static_cast<int>(ln_even((a.M + teams - 1) / teams, most, teams, odd ? ln_period(a.N, K::P) : 1));
+  l->plan.step = LnSteps(a, K::ESZ, static_cast<long long>(l->parts) * teams);
   return a.M / teams / l->parts < (1 << 30);
 }
 
