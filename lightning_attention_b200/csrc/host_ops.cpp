@@ -402,20 +402,19 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     LnSaved s;
     Tensor y = layer_norm_forward(x, g, w, b, eps, save8, &s);
     ctx->save_for_backward({s.x, s.xs, s.g, s.gs, s.stats, w, g.defined() ? b : Tensor()});
-    ctx->saved_data["rows"] = x.numel() / x.size(-1);
-    ctx->saved_data["width"] = x.size(-1);
-    ctx->saved_data["type"] = static_cast<int64_t>(x.scalar_type());
-    ctx->saved_data["params"] = static_cast<int64_t>(w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : at::kFloat);
-    // which tensors there were, in the order of the node's inputs
-    ctx->saved_data["given"] = (g.defined() ? 1 : 0) | (w.defined() ? 2 : 0) | (b.defined() ? 4 : 0) | (save8 ? 8 : 0);
+    const auto ptype = w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : at::kFloat;
+    // rows, their width, the types, and which tensors there were, in the order of the node's inputs
+    ctx->saved_data["call"] = std::vector<int64_t>{x.numel() / x.size(-1), x.size(-1), static_cast<int64_t>(x.scalar_type()), static_cast<int64_t>(ptype),
+                                                   (g.defined() ? 1 : 0) | (w.defined() ? 2 : 0) | (b.defined() ? 4 : 0) | (save8 ? 8 : 0)};
     return y;
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     TORCH_CHECK(!at::GradMode::is_enabled(), "layer norm can be differentiated once only: its backward pass does not run with create_graph=True");
     const variable_list saved = ctx->get_saved_variables();
-    const int64_t M = ctx->saved_data["rows"].toInt(), N = ctx->saved_data["width"].toInt(), given = ctx->saved_data["given"].toInt();
-    const auto type = static_cast<at::ScalarType>(ctx->saved_data["type"].toInt()), ptype = static_cast<at::ScalarType>(ctx->saved_data["params"].toInt());
+    const auto call = ctx->saved_data["call"].toIntList();
+    const int64_t M = call[0], N = call[1], given = call[4];
+    const auto type = static_cast<at::ScalarType>(static_cast<int64_t>(call[2])), ptype = static_cast<at::ScalarType>(static_cast<int64_t>(call[3]));
     const bool gated = given & 1, save8 = given & 8;
     Tensor dy = grads[0];
     TORCH_CHECK(dy.numel() == M * N && dy.size(-1) == N, "gradient and input sizes differ");

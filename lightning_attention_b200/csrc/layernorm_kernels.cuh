@@ -513,8 +513,9 @@ __global__ void __launch_bounds__((LN_FWD_THREADS<GATE, SAVE>)) ln_fwd_kernel(co
       if ((t & 31) == 0) slot[warp] = make_float4(m + mean, squares, fcount, 0.f);
       asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(T) : "memory");
       float total = 0.f, both = 0.f;
+      constexpr int AT_ONCE = SAVE ? 4 : 2;  // without checkpoints, four spill
       const auto join = [&](int from, int to) {
-#pragma unroll
+#pragma unroll AT_ONCE
         for (int w = from; w < to; ++w) {
           const float d = slot[w].x - m, zd = slot[w].z * d;
           total += zd;

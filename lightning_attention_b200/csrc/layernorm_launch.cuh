@@ -9,7 +9,7 @@ namespace lab200 {
 
 constexpr int LN_MAX_PARTS = 320;  // parts of dw and db: at most two CTAs for each SM, and a few to spare
 
-struct LnPlace { int sms; cudaStream_t st; };
+struct LnPlace { int device, sms; cudaStream_t st; };  // the current device, its SMs
 
 template <int DT> cudaError_t ln_fwd(const LnArgs& a, LnPlace at);
 template <int DT> cudaError_t ln_bwd(LnArgs a, LnPlace at);  // sets a.nparts; does not join the parts

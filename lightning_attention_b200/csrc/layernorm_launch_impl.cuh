@@ -1,4 +1,6 @@
 #pragma once
+#include <atomic>
+
 #include "layernorm_launch.cuh"
 
 namespace lab200 {
@@ -42,15 +44,27 @@ inline long long ln_even(long long ctas, long long most, int teams, int period) 
   return ctas <= most ? ctas : most / unit * unit > 0 ? most / unit * unit : unit;
 }
 
-template <class Kern, class Plan>
-cudaError_t ln_launch(Kern kern, unsigned grid, int cta, size_t shared, cudaStream_t st, const LnArgs& a, const Plan& plan) {
-  cudaError_t rc = shared > 40 * 1024 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared)) : cudaSuccess;
-  if (rc == cudaSuccess) {
-    kern<<<grid, cta, shared, st>>>(a, plan);
-    count_launch();
+// Static shared memory that a kernel may have beside its dynamic part.
+constexpr int LN_STATIC = 640 / 64 * 2 * (640 / 32) * 16;
+
+// KERN has had its limit of dynamic shared memory raised on the devices whose bits are set.
+template <auto KERN>
+std::atomic<unsigned long long> ln_raised{0};
+
+template <auto KERN, class Plan>
+cudaError_t ln_launch(unsigned grid, int cta, size_t shared, LnPlace at, const LnArgs& a, const Plan& plan) {
+  const unsigned long long bit = at.device < 64 ? 1ull << at.device : 0;
+  if (!(ln_raised<KERN>.load(std::memory_order_relaxed) & bit)) {
+    const cudaError_t rc = cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, LN_SHARED - LN_STATIC);
+    if (rc != cudaSuccess) {
+      cudaGetLastError();
+      return rc;
+    }
+    ln_raised<KERN>.fetch_or(bit, std::memory_order_relaxed);
   }
-  const cudaError_t last = cudaGetLastError();
-  return rc == cudaSuccess ? last : rc;
+  KERN<<<grid, cta, shared, at.st>>>(a, plan);
+  count_launch();
+  return cudaGetLastError();
 }
 
 template <int DT>
@@ -65,8 +79,7 @@ cudaError_t ln_fwd_team(const LnArgs& a, LnPlace at, int T) {
   const bool gate = a.gate, save = a.xcodes;
   const int threads = gate && save ? LN_FWD_THREADS<true, true> : LN_FWD_THREADS<false, false>, teams = threads / T, cta = teams * T, stage = threads * 16 * V * (gate ? 2 : 1);
   const size_t planes = ODD ? 0 : static_cast<size_t>(a.N) * 8;
-  // beside the kernel's slots
-  constexpr size_t room = LN_SHARED - (G > 32 ? 640 / 64 * 2 * (640 / 32) * 16 : 640);
+  constexpr size_t room = LN_SHARED - LN_STATIC;
   int stages = planes > room ? 0 : static_cast<int>((room - planes) / stage);
   if (stages < 2) return ln_fwd_any<DT>(a, at);
   stages = stages > 4 ? 4 : stages;
@@ -74,13 +87,13 @@ cudaError_t ln_fwd_team(const LnArgs& a, LnPlace at, int T) {
   const unsigned grid = static_cast<unsigned>(ln_even((a.M + teams - 1) / teams, at.sms, teams, ODD ? ln_period(a.N, LnPack<DT>::P) : 1));
   const LnFwdPlan plan{T, stages, LnSteps(a, LnPack<DT>::ESZ, static_cast<long long>(grid) * teams)};
   if constexpr (ODD) {
-    return gate ? ln_launch(ln_fwd_kernel<DT, V, G, true, true, false>, grid, cta, shared, at.st, a, plan)
-                : ln_launch(ln_fwd_kernel<DT, V, G, true, false, false>, grid, cta, shared, at.st, a, plan);
+    return gate ? ln_launch<ln_fwd_kernel<DT, V, G, true, true, false>>(grid, cta, shared, at, a, plan)
+                : ln_launch<ln_fwd_kernel<DT, V, G, true, false, false>>(grid, cta, shared, at, a, plan);
   } else {
-    if (gate) return save ? ln_launch(ln_fwd_kernel<DT, V, G, false, true, true>, grid, cta, shared, at.st, a, plan)
-                          : ln_launch(ln_fwd_kernel<DT, V, G, false, true, false>, grid, cta, shared, at.st, a, plan);
-    return save ? ln_launch(ln_fwd_kernel<DT, V, G, false, false, true>, grid, cta, shared, at.st, a, plan)
-                : ln_launch(ln_fwd_kernel<DT, V, G, false, false, false>, grid, cta, shared, at.st, a, plan);
+    if (gate) return save ? ln_launch<ln_fwd_kernel<DT, V, G, false, true, true>>(grid, cta, shared, at, a, plan)
+                          : ln_launch<ln_fwd_kernel<DT, V, G, false, true, false>>(grid, cta, shared, at, a, plan);
+    return save ? ln_launch<ln_fwd_kernel<DT, V, G, false, false, true>>(grid, cta, shared, at, a, plan)
+                : ln_launch<ln_fwd_kernel<DT, V, G, false, false, false>>(grid, cta, shared, at, a, plan);
   }
 }
 
@@ -129,7 +142,8 @@ bool ln_bwd_plan(const LnArgs& a, LnPlace at, LnBwdLaunch* l) {
   const size_t fixed = (l->G > 32 ? LN_BWD_SLOTS : 0) + (gate && !odd && K::P == 8 ? static_cast<size_t>(4) * LN_BWD_THREADS * V * 16 : 0);
   const int units = l->cta / (l->G <= 32 ? 32 : T);
   const size_t sums = odd ? static_cast<size_t>(a.N) * 4 : static_cast<size_t>(units - 1) * E * T * 4;
-  const int stages = fixed > LN_SHARED ? 0 : static_cast<int>((LN_SHARED - fixed) / stage);
+  constexpr size_t room = LN_SHARED - LN_STATIC;
+  const int stages = fixed > room ? 0 : static_cast<int>((room - fixed) / stage);
   if (stages < 2) return false;
   l->plan.T = T;
   l->plan.stages = stages > 4 ? 4 : stages;
@@ -145,10 +159,10 @@ template <int DT, int G, bool ODD>
 cudaError_t ln_bwd_team(const LnArgs& a, LnPlace at, const LnBwdLaunch& l) {
   const bool gate = a.gate || a.gcodes, saved = a.xcodes;
   constexpr int E = 16, EG = ODD ? 8 : 16;
-  if (gate) return saved ? ln_launch(ln_bwd_kernel<DT, EG, G, ODD, true, true>, l.parts, l.cta, l.shared, at.st, a, l.plan)
-                         : ln_launch(ln_bwd_kernel<DT, EG, G, ODD, true, false>, l.parts, l.cta, l.shared, at.st, a, l.plan);
-  return saved ? ln_launch(ln_bwd_kernel<DT, E, G, ODD, false, true>, l.parts, l.cta, l.shared, at.st, a, l.plan)
-               : ln_launch(ln_bwd_kernel<DT, E, G, ODD, false, false>, l.parts, l.cta, l.shared, at.st, a, l.plan);
+  if (gate) return saved ? ln_launch<ln_bwd_kernel<DT, EG, G, ODD, true, true>>(l.parts, l.cta, l.shared, at, a, l.plan)
+                         : ln_launch<ln_bwd_kernel<DT, EG, G, ODD, true, false>>(l.parts, l.cta, l.shared, at, a, l.plan);
+  return saved ? ln_launch<ln_bwd_kernel<DT, E, G, ODD, false, true>>(l.parts, l.cta, l.shared, at, a, l.plan)
+               : ln_launch<ln_bwd_kernel<DT, E, G, ODD, false, false>>(l.parts, l.cta, l.shared, at, a, l.plan);
 }
 
 template <int DT>

@@ -3,6 +3,8 @@
 #include <cuda_runtime.h>
 #include <math.h>
 
+#include <atomic>
+
 #include "../../include/lightning_b200.h"
 #include "layernorm_launch.cuh"
 
@@ -22,10 +24,19 @@ bool size_ok(long long M, int N, long long ld) {
   return M >= 0 && N >= 1 && N <= (1 << 30) && widest <= (1LL << 58) && (M == 0 || widest <= (1LL << 58) / M);
 }
 
-int sm_count() {
-  int dev = 0, n = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  return n > 0 ? n : 148;
+// The current device and its number of SMs, which is asked for once.
+LnPlace place(cudaStream_t st) {
+  static std::atomic<int> known[64];
+  LnPlace at{0, 148, st};
+  if (cudaGetDevice(&at.device) != cudaSuccess) {
+    cudaGetLastError();
+    return at;
+  }
+  int n = at.device < 64 ? known[at.device].load(std::memory_order_relaxed) : 0;
+  if (n == 0 && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, at.device) == cudaSuccess && at.device < 64)
+    known[at.device].store(n, std::memory_order_relaxed);
+  if (n > 0) at.sms = n;
+  return at;
 }
 
 // How a call's rows are given out to warps: by packs of P values, or (P 0) by groups. Contiguous rows of whole groups are one row.
@@ -74,7 +85,7 @@ __global__ void __launch_bounds__(1024) ln_bwd_join_kernel(const float* __restri
 template <int DT>
 int run_bwd(LnArgs a, cudaStream_t st) {
   if (a.M > 0) {
-    const LnPlace at{sm_count(), st};
+    const LnPlace at = place(st);
     if (a.partial) a.nparts = ln_bwd_parts<DT>(a, at);
     if (ln_bwd<DT>(a, at) != cudaSuccess) return LAB200_ERR_CUDA;
   }
@@ -102,7 +113,7 @@ int lab200_layernorm_fwd(const void* x, long long ldx, const void* gate, long lo
   a.M = M; a.N = N; a.eps = eps;
   if (reinterpret_cast<uintptr_t>(stats) & 7) return LAB200_ERR_ALIGN;
   a.vec_params = aligned_params(a);
-  const LnPlace at{sm_count(), static_cast<cudaStream_t>(stream)};
+  const LnPlace at = place(static_cast<cudaStream_t>(stream));
   // groups of 32 values do not keep to the packs of odd rows: those are checkpointed on their own
   if (xcodes && N % (dtype == LAB200_F32 ? 4 : 8)) {
     int rc = lab200_pack8(x, ldx, xcodes, xscales, M, N, dtype, stream);
@@ -159,7 +170,7 @@ int lab200_pack8(const void* x, long long ldx, void* codes, void* scales, long l
   const bool packs = !((reinterpret_cast<uintptr_t>(x) | static_cast<uintptr_t>(ldx) * esz | static_cast<uintptr_t>(N) * esz) & 15) &&
                      !(reinterpret_cast<uintptr_t>(codes) % (16 / esz));
   const PkRows r = pk_rows(M, N, packs ? 16 / esz : 0, ldx == N);
-  const unsigned grid = ln_capped((r.items + 7) / 8, 16LL * sm_count());
+  const unsigned grid = ln_capped((r.items + 7) / 8, 16LL * place(st).sms);
 #define LAB200_PACK(DT) \
   packs ? pack8_kernel<DT, PK_U><<<grid, 256, 0, st>>>(x, ldx, c, s, r) : pack8_any_kernel<DT, PK_U><<<grid, 256, 0, st>>>(x, ldx, c, s, N, r)
   if (dtype == LAB200_F32) LAB200_PACK(SRMS_F32);
@@ -180,7 +191,7 @@ int lab200_unpack8(const void* codes, const void* scales, void* y, long long M, 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool packs = !((reinterpret_cast<uintptr_t>(y) | static_cast<uintptr_t>(N) * esz) & 15) && !(reinterpret_cast<uintptr_t>(codes) % (16 / esz));
   const PkRows r = pk_rows(M, N, packs ? 16 / esz : 0, true);
-  const unsigned grid = ln_capped((r.items + 7) / 8, 16LL * sm_count());
+  const unsigned grid = ln_capped((r.items + 7) / 8, 16LL * place(st).sms);
 #define LAB200_UNPACK(DT) \
   packs ? unpack8_kernel<DT, PK_U><<<grid, 256, 0, st>>>(c, s, y, r) : unpack8_any_kernel<DT, PK_U><<<grid, 256, 0, st>>>(c, s, y, N, r)
   if (dtype == LAB200_F32) LAB200_UNPACK(SRMS_F32);
