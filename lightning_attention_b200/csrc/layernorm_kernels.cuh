@@ -927,26 +927,37 @@ __global__ void __launch_bounds__(LN_BWD_THREADS) ln_bwd_kernel(const LnArgs a, 
   if (!a.partial) return;
   float* sums = reinterpret_cast<float*>(ln_shared);
   if constexpr (ODD) {
-    // The CTA's part of dw and db: teams have columns of their own in a pack, so their sums meet by column in shared memory, one
-    // team after the other.
-#pragma unroll
+    // The CTA's part of dw and db: teams have columns of their own in a pack, so their sums meet by column in shared memory. A number of
+    // threads add up a column's teams, each every so-manieth one, and one of them these in turn.
+    const int parts = N < lanes ? min(lanes / N, teams) : 1;
     for (int which = 0; which < 2; ++which) {
-      for (int k = 0; k < teams; ++k) {
-        __syncthreads();
-        if (team == k)
+      __syncthreads();
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            float f[P];
-            K::floats(which ? db[i] : dw[i], f);
+      for (int i = 0; i < V; ++i) {
+        float f[P];
+        f2 both[H];
 #pragma unroll
-            for (int e = 0; e < P; ++e) {
-              const int col = (t + i * T) * P - shift + e;
-              if (col >= 0 && col < N) sums[col] = k ? sums[col] + f[e] : f[e];
-            }
-          }
+        for (int j = 0; j < H; ++j) both[j] = which ? db[i][j] : dw[i][j];
+        K::floats(both, f);
+#pragma unroll
+        for (int e = 0; e < P; ++e) {
+          const int col = (t + i * T) * P - shift + e;
+          if (col >= 0 && col < N) sums[team * N + col] = f[e];
+        }
       }
       __syncthreads();
-      for (int col = threadIdx.x; col < N; col += lanes) a.partial[(static_cast<size_t>(blockIdx.x) * 2 + which) * N + col] = sums[col];
+      for (int c = threadIdx.x; c < parts * N; c += lanes) {
+        const int part = c / N, col = c - part * N;
+        float sum = 0.f;
+        for (int k = part; k < teams; k += parts) sum += sums[k * N + col];
+        sums[part * N + col] = sum;  // team `part` is this thread's alone
+      }
+      __syncthreads();
+      for (int col = threadIdx.x; col < N; col += lanes) {
+        float sum = 0.f;
+        for (int k = 0; k < parts; ++k) sum += sums[k * N + col];
+        a.partial[(static_cast<size_t>(blockIdx.x) * 2 + which) * N + col] = sum;
+      }
     }
     return;
   }

@@ -105,6 +105,7 @@ cudaError_t ln_fwd(const LnArgs& a, LnPlace at) {
   if (kind == LN_ODD && !a.xcodes) {
     constexpr int V = 16 / K::P;
     const int npack = (a.N + 2 * K::P - 2) / K::P;  // of the row that begins last in its first pack
+    if (npack <= 4 * V) return ln_fwd_team<DT, V, 4, true>(a, at, 4);
     if (npack <= 8 * V) return ln_fwd_team<DT, V, 8, true>(a, at, 8);
     if (npack <= 32 * V) return ln_fwd_team<DT, V, 32, true>(a, at, 32);
     if (npack <= 512 * V) return ln_fwd_team<DT, V, 64, true>(a, at, team(npack, V));
@@ -113,7 +114,9 @@ cudaError_t ln_fwd(const LnArgs& a, LnPlace at) {
   if (kind != LN_PACKS || npack > 512 * 4) return ln_fwd_any<DT>(a, at);
   if (npack <= 512 && a.M * team(npack, 4) < 148 * 256)
     return npack <= 32 ? ln_fwd_team<DT, 1, 32, false>(a, at, 32) : ln_fwd_team<DT, 1, 64, false>(a, at, team(npack, 1));
-  if (npack <= 16 && K::LANES <= 4) return ln_fwd_team<DT, 4, 4, false>(a, at, 4);
+  if (npack <= K::LANES) return ln_fwd_team<DT, 1, K::LANES, false>(a, at, K::LANES);
+  if (npack <= 2 * K::LANES) return ln_fwd_team<DT, 2, K::LANES, false>(a, at, K::LANES);
+  if (npack <= 16) return ln_fwd_team<DT, 16 / K::LANES, K::LANES, false>(a, at, K::LANES);
   if (npack <= 32) return ln_fwd_team<DT, 4, 8, false>(a, at, 8);
   if (npack <= 64) return ln_fwd_team<DT, 4, 16, false>(a, at, 16);
   if (npack <= 128) return ln_fwd_team<DT, 4, 32, false>(a, at, 32);
@@ -134,14 +137,14 @@ bool ln_bwd_plan(const LnArgs& a, LnPlace at, LnBwdLaunch* l) {
   const auto team = [&](int e) { return (npack + e / K::P * 32 - 1) / (e / K::P * 32) * 32; };
   const int E = odd && gate ? 8 : 16, V = E / K::P;
   if (npack > LN_BWD_THREADS * V) return false;
-  l->G = npack <= 8 * V ? 8 : npack <= 16 * V ? 16 : npack <= 32 * V ? 32 : 64;
+  l->G = npack <= 2 * V ? 2 : npack <= 4 * V ? 4 : npack <= 8 * V ? 8 : npack <= 16 * V ? 16 : npack <= 32 * V ? 32 : 64;
   const int T = l->G <= 32 ? l->G : team(E), teams = LN_BWD_THREADS / T;
   l->cta = teams * T;
   const size_t in = static_cast<size_t>(V) * LN_BWD_THREADS * (saved ? K::P : 16), stage = static_cast<size_t>(V) * LN_BWD_THREADS * 16 + in * (gate ? 2 : 1);
   // the kernel's slots and planes
   const size_t fixed = (l->G > 32 ? LN_BWD_SLOTS : 0) + (gate && !odd && K::P == 8 ? static_cast<size_t>(4) * LN_BWD_THREADS * V * 16 : 0);
   const int units = l->cta / (l->G <= 32 ? 32 : T);
-  const size_t sums = odd ? static_cast<size_t>(a.N) * 4 : static_cast<size_t>(units - 1) * E * T * 4;
+  const size_t sums = odd ? static_cast<size_t>(teams) * a.N * 4 : static_cast<size_t>(units - 1) * E * T * 4;
   constexpr size_t room = LN_SHARED - LN_STATIC;
   const int stages = fixed > room ? 0 : static_cast<int>((room - fixed) / stage);
   if (stages < 2) return false;
@@ -165,6 +168,18 @@ cudaError_t ln_bwd_team(const LnArgs& a, LnPlace at, const LnBwdLaunch& l) {
                : ln_launch<ln_bwd_kernel<DT, E, G, ODD, false, false>>(l.parts, l.cta, l.shared, at, a, l.plan);
 }
 
+template <int DT, bool ODD>
+cudaError_t ln_bwd_teams(const LnArgs& a, LnPlace at, const LnBwdLaunch& l) {
+  switch (l.G) {
+    case 2: return ln_bwd_team<DT, 2, ODD>(a, at, l);
+    case 4: return ln_bwd_team<DT, 4, ODD>(a, at, l);
+    case 8: return ln_bwd_team<DT, 8, ODD>(a, at, l);
+    case 16: return ln_bwd_team<DT, 16, ODD>(a, at, l);
+    case 32: return ln_bwd_team<DT, 32, ODD>(a, at, l);
+    default: return ln_bwd_team<DT, 64, ODD>(a, at, l);
+  }
+}
+
 template <int DT>
 int ln_bwd_parts(const LnArgs& a, LnPlace at) {
   LnBwdLaunch l;
@@ -175,11 +190,7 @@ template <int DT>
 cudaError_t ln_bwd(LnArgs a, LnPlace at) {
   LnBwdLaunch l;
   if (ln_bwd_plan<DT>(a, at, &l)) {
-    if (l.kind == LN_ODD)
-      return l.G == 8 ? ln_bwd_team<DT, 8, true>(a, at, l) : l.G == 16 ? ln_bwd_team<DT, 16, true>(a, at, l)
-           : l.G == 32 ? ln_bwd_team<DT, 32, true>(a, at, l) : ln_bwd_team<DT, 64, true>(a, at, l);
-    return l.G == 8 ? ln_bwd_team<DT, 8, false>(a, at, l) : l.G == 16 ? ln_bwd_team<DT, 16, false>(a, at, l)
-         : l.G == 32 ? ln_bwd_team<DT, 32, false>(a, at, l) : ln_bwd_team<DT, 64, false>(a, at, l);
+    return l.kind == LN_ODD ? ln_bwd_teams<DT, true>(a, at, l) : ln_bwd_teams<DT, false>(a, at, l);
   }
   if (a.dx || a.dgate) {
     ln_bwd_any_kernel<DT><<<ln_capped(a.M, 1 << 20), 256, 0, at.st>>>(a);

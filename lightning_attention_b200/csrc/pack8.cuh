@@ -87,9 +87,14 @@ __device__ __forceinline__ unsigned long long pk_two(uint32_t w, int e) {
 }
 
 // ---- pack and unpack on their own: streaming kernels, bound by memory (3 1/32 bytes for each 16-bit value) -----------------------
-// Where packs of 16 bytes divide the rows: a warp takes 32 * U adjacent packs of a row at a time, a lane every 32nd, so that LANES
-// adjacent lanes hold a group and U accesses are under way. `npack` packs to a row; contiguous rows of whole groups come as one row.
-struct PkRows { long long M, npack, ngroups, items; int per_row; };
+// Where packs of 16 bytes divide the rows, a thread has U packs, 32 apart, so that adjacent lanes hold a group and U accesses are under
+// way. Contiguous rows of whole groups count as one row; otherwise rows are counted in whole groups, the last one's missing packs
+// included, and a pack's row comes from a multiplication (`magic`) in place of a division. Past 2^31 packs a warp stays in one row.
+struct PkRows {
+  long long M, npack, ngroups, items;  // packs (without: groups) of a row, its groups; what warps take at a time
+  int per_row;                         // items of a row
+  uint32_t units, magic, shift;        // packs of a row counted in whole groups; 0: a warp stays in one row
+};
 
 __device__ __forceinline__ void pk_item(const PkRows& r, long long item, long long* row, long long* k) {
   if (r.M == 1) {
@@ -103,28 +108,44 @@ __device__ __forceinline__ void pk_item(const PkRows& r, long long item, long lo
     *k = item - *row * r.per_row;
   }
 }
+// Where a thread's packs of an item are: row and number of pack i, npack or more where there is none. UNITS: r.units is given.
+template <int U, bool UNITS>
+struct PkPlaces {
+  long long row, k0;
+  uint32_t q0;
+  __device__ PkPlaces(const PkRows& r, long long item, int lane) {
+    if constexpr (UNITS) {
+      q0 = static_cast<uint32_t>(item) * (32 * U) + lane;
+    } else {
+      pk_item(r, item, &row, &k0);
+      k0 = k0 * (32 * U) + lane;
+    }
+  }
+  __device__ long long row_of(const PkRows& r, int i) const { return UNITS ? __umulhi(q0 + 32 * i, r.magic) >> r.shift : row; }
+  __device__ long long pack_of(const PkRows& r, int i) const {
+    if constexpr (!UNITS) return k0 + 32 * i;
+    const uint32_t y = __umulhi(q0 + 32 * i, r.magic) >> r.shift;
+    return y < r.M ? q0 + 32 * i - y * r.units : static_cast<uint32_t>(r.npack);
+  }
+};
 
-template <int DT, int U>
+template <int DT, int U, bool UNITS>
 __global__ void __launch_bounds__(256)
 pack8_kernel(const void* __restrict__ x_, long long ldx, int8_t* __restrict__ codes, uint8_t* __restrict__ scales, const PkRows r) {
   constexpr int P = SrmsVec<DT>::EPV, LANES = PK_GROUP / P, ESZ = 16 / P;
   const int lane = threadIdx.x & 31;
   const long long step = static_cast<long long>(gridDim.x) * 8;
   for (long long item = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5); item < r.items; item += step) {
-    long long row, k0;
-    pk_item(r, item, &row, &k0);
-    k0 = k0 * (32 * U) + lane;
-    const auto* x = reinterpret_cast<const SrmsPack<1>*>(static_cast<const char*>(x_) + row * ldx * ESZ);
+    const PkPlaces<U, UNITS> at(r, item, lane);
     SrmsPack<1> v[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
+      const long long k = at.pack_of(r, i);
       v[i].q[0] = make_uint4(0, 0, 0, 0);
-      if (k0 + 32 * i < r.npack) v[i] = ld_stream<1>(x + k0 + 32 * i);
+      if (k < r.npack) v[i] = ld_stream<1>(reinterpret_cast<const SrmsPack<1>*>(static_cast<const char*>(x_) + at.row_of(r, i) * ldx * ESZ) + k);
     }
-    auto* to = reinterpret_cast<uint32_t*>(codes + row * r.npack * P);
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const long long k = k0 + 32 * i;
       float f[P];
       SrmsVec<DT>::unpack(v[i].q[0], f);
       unsigned long long two[P / 2];
@@ -133,7 +154,9 @@ pack8_kernel(const void* __restrict__ x_, long long ldx, int8_t* __restrict__ co
       const uint32_t e = pk_pack_exponent<DT>(v[i].q[0]);
       uint32_t w[P / 4];
       pk_pack_codes<P>(two, e, w);
+      const long long row = at.row_of(r, i), k = at.pack_of(r, i);
       if (k < r.npack) {
+        auto* to = reinterpret_cast<uint32_t*>(codes + row * r.npack * P);
         if constexpr (P == 8) reinterpret_cast<uint2*>(to)[k] = make_uint2(w[0], w[1]);
         else to[k] = w[0];
         if (k % LANES == 0) scales[row * r.ngroups + k / LANES] = static_cast<uint8_t>(e);
@@ -142,23 +165,20 @@ pack8_kernel(const void* __restrict__ x_, long long ldx, int8_t* __restrict__ co
   }
 }
 
-template <int DT, int U>
+template <int DT, int U, bool UNITS>
 __global__ void __launch_bounds__(256)
 unpack8_kernel(const int8_t* __restrict__ codes, const uint8_t* __restrict__ scales, void* __restrict__ y_, const PkRows r) {
   constexpr int P = SrmsVec<DT>::EPV, LANES = PK_GROUP / P;
   const int lane = threadIdx.x & 31;
   const long long step = static_cast<long long>(gridDim.x) * 8;
   for (long long item = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5); item < r.items; item += step) {
-    long long row, k0;
-    pk_item(r, item, &row, &k0);
-    k0 = k0 * (32 * U) + lane;
-    const auto* from = reinterpret_cast<const uint32_t*>(codes + row * r.npack * P);
-    auto* y = reinterpret_cast<SrmsPack<1>*>(y_) + row * r.npack;
+    const PkPlaces<U, UNITS> at(r, item, lane);
     uint32_t w[U][P / 4], e[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const long long k = k0 + 32 * i;
+      const long long row = at.row_of(r, i), k = at.pack_of(r, i);
       if (k < r.npack) {
+        const auto* from = reinterpret_cast<const uint32_t*>(codes + row * r.npack * P);
         if constexpr (P == 8) {
           const uint2 v = __ldcs(reinterpret_cast<const uint2*>(from) + k);
           w[i][0] = v.x; w[i][P / 4 - 1] = v.y;
@@ -170,7 +190,7 @@ unpack8_kernel(const int8_t* __restrict__ codes, const uint8_t* __restrict__ sca
     }
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const long long k = k0 + 32 * i;
+      const long long row = at.row_of(r, i), k = at.pack_of(r, i);
       if (k < r.npack) {
         const float unit = pk_step(e[i]);
         float f[P];
@@ -184,7 +204,7 @@ unpack8_kernel(const int8_t* __restrict__ codes, const uint8_t* __restrict__ sca
         }
         SrmsPack<1> o;
         o.q[0] = SrmsVec<DT>::pack(f);
-        st_stream<1>(y + k, o);
+        st_stream<1>(reinterpret_cast<SrmsPack<1>*>(y_) + row * r.npack + k, o);
       }
     }
   }
