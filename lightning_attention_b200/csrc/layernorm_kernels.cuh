@@ -739,7 +739,7 @@ __global__ void __launch_bounds__(LN_BWD_THREADS) ln_bwd_kernel(const LnArgs a, 
   constexpr bool FILL = G < 32;
   // Weight and bias: in registers, or, with a gate, where these would not do: in shared memory (PLANES), or, in fp32, where that would not
   // either, read again for each row.
-  constexpr bool PLANES = GATE && !ODD && DT != SRMS_F32, AGAIN = GATE && !ODD && !PLANES, HELD = !PLANES && !AGAIN;
+  constexpr bool PLANES = GATE && !ODD && (DT != SRMS_F32 || SAVED), AGAIN = GATE && !ODD && !PLANES, HELD = !PLANES && !AGAIN;
   using In = LnRows<DT, V, ODD, SAVED>;
   using Dy = LnRows<DT, V, ODD, false>;
   constexpr uint32_t STAGE = Dy::BYTES + In::BYTES * (GATE ? 2 : 1), SLOTS = G > 32 ? LN_BWD_SLOTS : 0;

@@ -142,7 +142,7 @@ bool ln_bwd_plan(const LnArgs& a, LnPlace at, LnBwdLaunch* l) {
   l->cta = teams * T;
   const size_t in = static_cast<size_t>(V) * LN_BWD_THREADS * (saved ? K::P : 16), stage = static_cast<size_t>(V) * LN_BWD_THREADS * 16 + in * (gate ? 2 : 1);
   // the kernel's slots and planes
-  const size_t fixed = (l->G > 32 ? LN_BWD_SLOTS : 0) + (gate && !odd && K::P == 8 ? static_cast<size_t>(4) * LN_BWD_THREADS * V * 16 : 0);
+  const size_t fixed = (l->G > 32 ? LN_BWD_SLOTS : 0) + (gate && !odd && (K::P == 8 || saved) ? static_cast<size_t>(2 * K::P / 4) * LN_BWD_THREADS * V * 16 : 0);
   const int units = l->cta / (l->G <= 32 ? 32 : T);
   const size_t sums = odd ? static_cast<size_t>(teams) * a.N * 4 : static_cast<size_t>(units - 1) * E * T * 4;
   constexpr size_t room = LN_SHARED - LN_STATIC;

@@ -220,17 +220,23 @@ pack8_any_kernel(const void* __restrict__ x_, long long ldx, int8_t* __restrict_
   for (long long item = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5); item < r.items; item += step) {
     long long row, k0;
     pk_item(r, item, &row, &k0);
-    const auto* x = static_cast<const typename E::T*>(x_) + row * ldx;
     const int g0 = static_cast<int>(k0) * U, c0 = g0 * PK_GROUP + lane;
+    const auto* x = static_cast<const typename E::T*>(x_) + row * ldx + c0;
+    int8_t* to = codes + row * N + c0;
+    uint8_t* to_scales = scales + row * r.ngroups + g0;
     float v[U];
 #pragma unroll
-    for (int i = 0; i < U; ++i) v[i] = c0 + i * PK_GROUP < N ? E::ld(x + c0 + i * PK_GROUP) : 0.f;
+    for (int i = 0; i < U; ++i) v[i] = c0 + i * PK_GROUP < N ? E::ld(x + i * PK_GROUP) : 0.f;
+    uint32_t mine = 0;  // lane i keeps the exponent of group i
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const uint32_t e = pk_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(v[i]))));
-      if (c0 + i * PK_GROUP < N) codes[row * N + c0 + i * PK_GROUP] = static_cast<int8_t>(pk_code(v[i], pk_inv_step(e)));
-      if (lane == 0 && g0 + i < r.ngroups) scales[row * r.ngroups + g0 + i] = static_cast<uint8_t>(e);
+      // as in pk_pack_codes
+      const int code = e < 254u ? __float_as_int(fmaf(v[i], pk_inv_step(e), 12582912.f)) : pk_code(v[i], pk_inv_step(e));
+      if (c0 + i * PK_GROUP < N) to[i * PK_GROUP] = static_cast<int8_t>(code);
+      if (lane == i) mine = e;
     }
+    if (lane < U && g0 + lane < r.ngroups) to_scales[lane] = static_cast<uint8_t>(mine);
   }
 }
 

@@ -20,6 +20,16 @@ def rows(t, N):
     return t, (t.stride(0) if M > 1 else N)
 
 
+def packed_rows(t, N):
+    """The same for the layer norms, whose fast kernels read the rows of a contiguous tensor that begins on 16 bytes, or whole packs of
+    16 bytes: other rows are copied, which costs less than reading them value by value."""
+    t, ld = rows(t, N)
+    size = t.element_size()
+    if t.data_ptr() % 16 or (ld != N and (N * size % 16 or ld * size % 16)):
+        t, ld = t.clone(memory_format=torch.contiguous_format), N
+    return t, ld
+
+
 def scales_shape(shape):
     return (*shape[:-1], -(-shape[-1] // GROUP))
 

@@ -6,7 +6,7 @@ With `save_8bit` the backward pass keeps x (and the gate) as 8-bit checkpoints, 
 import torch
 
 from ... import _lib
-from .checkpoint8 import checkpoint_fits, differentiable_once, empty_checkpoint, rows
+from .checkpoint8 import checkpoint_fits, differentiable_once, empty_checkpoint, packed_rows
 
 
 def _check(x, gate, weight, bias, eps):
@@ -36,8 +36,8 @@ class _LayerNorm(torch.autograd.Function):
     def forward(ctx, x, gate, weight, bias, eps, save_8bit, wanted):
         _check(x, gate, weight, bias, eps)
         shape, N = x.shape, x.shape[-1]
-        x2, ldx = rows(x, N)
-        g2, ldg = rows(gate, N) if gate is not None else (None, N)
+        x2, ldx = packed_rows(x, N)
+        g2, ldg = packed_rows(gate, N) if gate is not None else (None, N)
         weight, bias = _contiguous(weight), _contiguous(bias)
         M = x2.shape[0]
         y = torch.empty(shape, dtype=x.dtype, device=x.device)
@@ -54,10 +54,8 @@ class _LayerNorm(torch.autograd.Function):
                 _lib.ptr(xc), _lib.ptr(xs), _lib.ptr(gc), _lib.ptr(gs), M, N, float(eps), _lib.dtype_code(x.dtype), _lib.stream_ptr(x.device))
         _lib.check(rc, "lab200_layernorm_fwd")
         if wanted:
-            # the tensors themselves where they are read in place, so that a change to them is noticed
-            keep = lambda t, t2: t if t is None or t2.data_ptr() == t.data_ptr() else t2
-            ctx.save_for_backward(*((xc, xs, gc, gs) if save_8bit else (keep(x, x2), None, keep(gate, g2), None)), stats, weight,
-                                  bias if gate is not None else None)
+            # the tensors themselves, not copies of other strides: a change to them is noticed
+            ctx.save_for_backward(*((xc, xs, gc, gs) if save_8bit else (x, None, gate, None)), stats, weight, bias if gate is not None else None)
             ctx.info = (M, N, x.dtype, x.device, gate is not None, wdt, bool(save_8bit))
         return y
 
@@ -78,14 +76,14 @@ class _LayerNorm(torch.autograd.Function):
         else:
             bad = bad or any(t.numel() != M * N or t.shape[-1] != N or t.dtype != dtype or t.device != device for t in ((first, second) if gated else (first,)))
             if not bad:
-                x2, ldx = rows(first, N)
-                g2, ldg = rows(second, N) if gated else (None, N)
+                x2, ldx = packed_rows(first, N)
+                g2, ldg = packed_rows(second, N) if gated else (None, N)
         if bad:
             raise RuntimeError("layer norm backward: saved-tensor hooks returned another shape, dtype or device")
         if dy.numel() != M * N:
             raise RuntimeError("gradient and input sizes differ")
         shape = dy.shape
-        dy2, lddy = rows(dy.to(dtype), N)
+        dy2, lddy = packed_rows(dy.to(dtype), N)
         stats, weight, bias = stats.contiguous(), _contiguous(weight), _contiguous(bias)
         new = lambda on, shape, dt: torch.empty(shape, dtype=dt, device=device) if on else None
         dx, dg, dw, db = new(need_x, shape, dtype), new(need_g, shape, dtype), new(need_w, (N,), wdt), new(need_b, (N,), wdt)

@@ -123,6 +123,77 @@ def test_strides(cuda_lib, m, n, dtype):
     assert y.shape == x3.shape and torch.autograd.grad(y, x3, dy.view_as(y))[0].shape == x3.shape
 
 
+@pytest.mark.parametrize("gated", [False, True], ids=["norm", "gate"])
+@pytest.mark.parametrize("m,n", [(5, 100), (3, 33), (4, 2052), (2, 12000), (40, 9)])
+def test_c_entry_reads_any_stride_and_alignment(cuda_lib, m, n, gated):
+    """lab200_layernorm_fwd / _bwd on rows that no pack of 16 bytes divides, which the Python operators copy."""
+    from lightning_attention_b200 import _lib
+
+    L = cuda_lib
+    x, gate, w, b, dy = inputs(m, n, torch.bfloat16, torch.float32, gated)
+    ref = reference(x, gate, w, b, EPS, dy)
+    ld = n + 3
+    wide = torch.full((3, m * ld + 1), float("nan"), device=DEV, dtype=torch.bfloat16)
+
+    def odd(k, t):
+        v = wide[k][1:].view(m, ld)[:, :n]
+        return v.copy_(t.detach())
+
+    xv, dyv = odd(0, x), odd(1, dy)
+    gv = odd(2, gate) if gated else None
+    y, dx, dg = (torch.full((m * n + 64,), 7.0, device=DEV, dtype=torch.bfloat16) for _ in range(3))
+    stats = torch.empty(m, 2, device=DEV)
+    dw, db = torch.empty(n, device=DEV), torch.empty(n, device=DEV)
+    s = torch.cuda.current_stream().cuda_stream
+    p = _lib.ptr
+    wd, bd = w.detach(), b.detach()
+    assert L.lab200_layernorm_fwd(p(xv), ld, p(gv), ld, p(wd), p(bd), _lib.F32, p(y), p(stats), None, None, None, None, m, n, EPS, _lib.BF16, s) == 0
+    nbytes = L.lab200_layernorm_bwd_workspace_bytes(m, n)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=DEV)
+    assert L.lab200_layernorm_bwd(p(xv), ld, p(gv), ld, None, None, None, None, p(stats), p(dyv), ld, p(wd), p(bd), _lib.F32, p(dx), p(dg) if gated else None, p(dw),
+                                  p(db), p(ws), nbytes, m, n, _lib.BF16, s) == 0
+    for name, t in (("y", y), ("dx", dx), *((("dgate", dg),) if gated else ())):
+        assert_within(t[:m * n].view(m, n), ref[name], name)
+        assert bool((t[m * n:] == 7).all()), f"{name}: written behind the last row"
+    assert_within(dw, ref["dw"], "dw")
+    assert_within(db, ref["db"], "db")
+
+
+@pytest.mark.parametrize("n", [33, 64, 100, 1001, 2048, 5120])
+@pytest.mark.parametrize("gated", [False, True], ids=["norm", "gate"])
+def test_nothing_is_written_outside_the_outputs(cuda_lib, n, gated):
+    """Guards around every output of the C entries, in both directions, with and without checkpoints."""
+    from lightning_attention_b200 import _lib
+
+    L, m = cuda_lib, 37
+    p = _lib.ptr
+    x, gate, w, b, dy = (None if t is None else t.detach() for t in inputs(m, n, torch.bfloat16, torch.float32, gated))
+    ng = (n + 31) // 32
+    s = torch.cuda.current_stream().cuda_stream
+
+    def guarded(count, dtype):
+        t = torch.full((count + 256,), 77, device=DEV, dtype=dtype)
+        return t, t[128:128 + count]
+
+    outs = {k: guarded(m * n, torch.bfloat16) for k in ("y", "dx", "dg")}
+    outs |= {"stats": guarded(2 * m, torch.float32), "dw": guarded(n, torch.float32), "db": guarded(n, torch.float32)}
+    outs |= {k: guarded(m * n, torch.int8) for k in ("xc", "gc")} | {k: guarded(m * ng, torch.uint8) for k in ("xs", "gs")}
+    o = {k: v[1].data_ptr() for k, v in outs.items()}
+    gcs = (o["gc"], o["gs"]) if gated else (None, None)
+    assert L.lab200_layernorm_fwd(p(x), n, p(gate), n, p(w), p(b), _lib.F32, o["y"], o["stats"], o["xc"], o["xs"], *gcs, m, n, EPS, _lib.BF16, s) == 0
+    nbytes = L.lab200_layernorm_bwd_workspace_bytes(m, n)
+    ws_all, ws = guarded(nbytes, torch.uint8)
+    for saved in (False, True):
+        src = (None, n, None, n, o["xc"], o["xs"], *gcs) if saved else (p(x), n, p(gate), n, None, None, None, None)
+        assert L.lab200_layernorm_bwd(*src, o["stats"], p(dy), n, p(w), p(b), _lib.F32, o["dx"], o["dg"] if gated else None, o["dw"], o["db"], ws.data_ptr(), nbytes,
+                                      m, n, _lib.BF16, s) == 0
+        ref = reference(x, gate, w, b, EPS, dy, saved)
+        assert_within(outs["dx"][1].view(m, n), ref["dx"], "dx")
+        assert_within(outs["dw"][1], ref["dw"], "dw")
+    for k, (whole, part) in list(outs.items()) + [("ws", (ws_all, ws))]:
+        assert bool((whole[:128] == 77).all()) and bool((whole[128 + part.numel():] == 77).all()), f"written outside {k}"
+
+
 def test_every_subset_of_gradients(cuda_lib):
     x, gate, w, b, dy = inputs(40, 192, torch.bfloat16, torch.float32, True)
     full = fwd_bwd(x, gate, w, b, dy)
