@@ -112,7 +112,10 @@ cudaError_t ln_fwd(const LnArgs& a, LnPlace at) {
   }
   const int npack = a.N / K::P;
   if (kind != LN_PACKS || npack > 512 * 4) return ln_fwd_any<DT>(a, at);
-  if (npack <= 512 && a.M * team(npack, 4) < 148 * 256)
+  // Rows of which one for each team of one pack a thread fills the GPU once or less: more threads to a row then cost less than they gain.
+  // Measured with one pack and with four, bf16: 1 x 2048 in 3.1 and 3.3 us, 296 x 2048 in 3.6 and 4.8, 888 x 2048 in 5.6 and 4.9;
+  // 888 x 768 in 3.7 and 3.9, 1184 x 768 in 4.6 and 3.9.
+  if (npack <= 512 && a.M * (npack <= 32 ? 32 : team(npack, 1)) <= at.sms * 640LL)
     return npack <= 32 ? ln_fwd_team<DT, 1, 32, false>(a, at, 32) : ln_fwd_team<DT, 1, 64, false>(a, at, team(npack, 1));
   if (npack <= K::LANES) return ln_fwd_team<DT, 1, K::LANES, false>(a, at, K::LANES);
   if (npack <= 2 * K::LANES) return ln_fwd_team<DT, 2, K::LANES, false>(a, at, K::LANES);
