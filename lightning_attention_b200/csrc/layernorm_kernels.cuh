@@ -48,8 +48,8 @@ __device__ __forceinline__ void ln_param_out(void* p, int wdt, int i, float v) {
 }
 
 // sigmoid(v) and sigmoid(-v) from -v / ln 2: 1 / (1 + e) and e / (1 + e), e = 2^(-v / ln 2) by the approximate instructions
-// (relative errors of 2^-22). Past 2^116 sigmoid(v) is nothing next to 1, so the bound changes no result and keeps inf * 0 out; it
-// lets a NaN pass.
+// (relative errors of 2^-22). The bound on e keeps inf * 0 out: with it sigmoid(v) stays at 2^-116 where it would go on to zero. A NaN
+// passes it.
 constexpr float LN_MINUS_LOG2E = -1.4426950408889634f;
 __device__ __forceinline__ void ln_sigmoid2(float arg, float* s, float* rest) {
   float e;
@@ -74,6 +74,8 @@ __device__ __forceinline__ float ln_saved(const void* p, long long ld, const int
 }
 
 // ---- rows of any length, stride and alignment: a CTA per row, element by element, each row read again for each sum ----------
+// For rows past what teams hold (8192 values and more) and for C callers' rows that the Python operators would copy. Bound by
+// instructions: 32768 x 4096 bf16 in 1040 us, both passes.
 template <int DT>
 __global__ void __launch_bounds__(256) ln_fwd_any_kernel(const LnArgs a) {
   using E = SrmsElem<DT>;

@@ -24,6 +24,13 @@ bool size_ok(long long M, int N, long long ld) {
   return M >= 0 && N >= 1 && N <= (1 << 30) && widest <= (1LL << 58) && (M == 0 || widest <= (1LL << 58) / M);
 }
 
+// Whether each pointer (NULL ones too) is a multiple of the size of what it points to.
+int size_of(int dtype) { return dtype == LAB200_F32 ? 4 : 2; }
+template <class... Ptr>
+bool whole(int size, Ptr... p) {
+  return ((reinterpret_cast<uintptr_t>(p) % size == 0) && ...);
+}
+
 // The current device and its number of SMs, which is asked for once.
 LnPlace place(cudaStream_t st) {
   static std::atomic<int> known[64];
@@ -50,7 +57,8 @@ PkRows pk_rows(long long M, long long N, int P, bool contiguous) {
   const long long units = P ? r.ngroups * (PK_GROUP / P) : r.ngroups, per = P ? 32 * PK_U : PK_U_ANY, per_row = (units + per - 1) / per;
   r.items = M * per_row;
   r.per_row = M == 1 ? 0 : static_cast<int>(per_row);
-  // rows that fill their last item well are left to warps, whose place costs less (20000 x 1000: 12 us, 15; 27408 x 312: XX, YY)
+  // rows that fill their last item well are left to warps, whose place costs less (20000 x 1000 in 12 us
+  // against 15; 27408 x 312 in 14 against 6, a warp having 40 packs for 128)
   if (P && M > 1 && units * 10 < per_row * per * 9 && M * units <= (1ll << 31) - per) {
     // n / d = umulhi(n, ceil(2^(31 + l) / d)) >> (l - 1) for n < 2^31 and 2^(l - 1) < d <= 2^l: the factor is too large by less
     // than d / 2^(31 + l), which n times stays below 1 / d
@@ -122,7 +130,7 @@ int lab200_layernorm_fwd(const void* x, long long ldx, const void* gate, long lo
   a.xcodes = static_cast<int8_t*>(xcodes); a.xscales = static_cast<uint8_t*>(xscales);
   a.gcodes = static_cast<int8_t*>(gcodes); a.gscales = static_cast<uint8_t*>(gscales);
   a.M = M; a.N = N; a.eps = eps;
-  if (reinterpret_cast<uintptr_t>(stats) & 7) return LAB200_ERR_ALIGN;
+  if (!whole(8, stats) || !whole(size_of(dtype), x, gate, y) || !whole(size_of(wdtype), weight, bias)) return LAB200_ERR_ALIGN;
   a.vec_params = aligned_params(a);
   const LnPlace at = place(static_cast<cudaStream_t>(stream));
   // groups of 32 values do not keep to the packs of odd rows: those are checkpointed on their own
@@ -152,7 +160,7 @@ int lab200_layernorm_bwd(const void* x, long long ldx, const void* gate, long lo
   if (M > 0 && (!stats || !dy || !x == !xcodes || !xcodes != !xscales || (gate && gcodes) || !gcodes != !gscales || (gate && xcodes) || (gcodes && x)))
     return LAB200_ERR_SHAPE;
   if (dgate && M > 0 && !gate && !gcodes) return LAB200_ERR_SHAPE;
-  if (reinterpret_cast<uintptr_t>(stats) & 7) return LAB200_ERR_ALIGN;
+  if (!whole(8, stats) || !whole(size_of(dtype), x, gate, dy, dx, dgate) || !whole(size_of(wdtype), weight, bias, dweight, dbias)) return LAB200_ERR_ALIGN;
   if ((dweight || dbias) && M > 0 && (!workspace || workspace_bytes < lab200_layernorm_bwd_workspace_bytes(M, N))) return LAB200_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return LAB200_ERR_ALIGN;
   LnArgs a = {};
@@ -173,8 +181,9 @@ int lab200_pack8(const void* x, long long ldx, void* codes, void* scales, long l
   if (!dtype_known(dtype)) return LAB200_ERR_DTYPE;
   if (M == 0) return LAB200_OK;
   if (!x || !codes || !scales) return LAB200_ERR_SHAPE;
+  const int esz = size_of(dtype);
+  if (!whole(esz, x)) return LAB200_ERR_ALIGN;
   if (M == 1) ldx = N;
-  const int esz = dtype == LAB200_F32 ? 4 : 2;
   auto* c = static_cast<int8_t*>(codes);
   auto* s = static_cast<uint8_t*>(scales);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -197,7 +206,8 @@ int lab200_unpack8(const void* codes, const void* scales, void* y, long long M, 
   if (!dtype_known(dtype)) return LAB200_ERR_DTYPE;
   if (M == 0) return LAB200_OK;
   if (!y || !codes || !scales) return LAB200_ERR_SHAPE;
-  const int esz = dtype == LAB200_F32 ? 4 : 2;
+  const int esz = size_of(dtype);
+  if (!whole(esz, y)) return LAB200_ERR_ALIGN;
   auto* c = static_cast<const int8_t*>(codes);
   auto* s = static_cast<const uint8_t*>(scales);
   cudaStream_t st = static_cast<cudaStream_t>(stream);

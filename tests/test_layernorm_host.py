@@ -53,7 +53,8 @@ def test_layernorm_fwd_argument_validation():
     assert fwd(eps=-1.0) == 1 and fwd(eps=float("nan")) == 1 and fwd(eps=float("inf")) == 1
     assert fwd(xc=p) == 1 and fwd(xs=p) == 1 and fwd(gc=p, gs=p) == 1  # half a checkpoint, a gate's without a gate
     assert fwd(gate=p, xc=p, xs=p) == 1 and fwd(gate=p, gc=p, gs=p) == 1  # both or none
-    assert fwd(stats=p + 4) == 6
+    assert fwd(stats=p + 4) == 6 and fwd(x=p + 1) == 6 and fwd(y=p + 1) == 6 and fwd(gate=p + 1) == 6
+    assert fwd(w=p + 1) == 6 and fwd(b=p + 2, w=None, wdt=_lib.F32) == 6
 
 
 def test_layernorm_bwd_argument_validation():
@@ -68,6 +69,7 @@ def test_layernorm_bwd_argument_validation():
     assert bwd(gate=p, gc=p, gs=p) == 1 and bwd(x=None, xc=p, xs=p, gate=p) == 1 and bwd(gc=p, gs=p) == 1
     assert bwd(stats=None) == 1 and bwd(dy=None) == 1 and bwd(dg=p) == 1
     assert bwd(dt=3) == 2 and bwd(wdt=_lib.F16) == 2
+    assert bwd(x=p + 1) == 6 and bwd(dy=p + 1) == 6 and bwd(dx=p + 1) == 6 and bwd(w=p + 1) == 6 and bwd(dw=p + 2, wdt=_lib.F32) == 6 and bwd(db=p + 1) == 6
     assert bwd(ws=None) == 3 and bwd(nbytes=8) == 3 and bwd(ws=p + 8) == 6 and bwd(stats=p + 4) == 6
     assert L.lab200_layernorm_bwd_workspace_bytes(0, 64) == 0
     sizes = [L.lab200_layernorm_bwd_workspace_bytes(m, 4096) for m in (1, 100, 4096, 1 << 20, 1 << 40)]
@@ -81,6 +83,7 @@ def test_pack8_argument_validation():
     assert L.lab200_pack8(None, 64, p, p, 2, 64, _lib.BF16, None) == 1 and L.lab200_pack8(p, 64, None, p, 2, 64, _lib.BF16, None) == 1
     assert L.lab200_pack8(p, 64, p, None, 2, 64, _lib.BF16, None) == 1 and L.lab200_pack8(p, 64, p, p, 2, 64, 3, None) == 2
     assert L.lab200_unpack8(p, p, p, -1, 64, _lib.BF16, None) == 1 and L.lab200_unpack8(p, p, p, 2, 64, 5, None) == 2
+    assert L.lab200_pack8(p + 1, 64, p, p, 2, 64, _lib.BF16, None) == 6 and L.lab200_unpack8(p, p, p + 2, 2, 64, _lib.F32, None) == 6
     assert L.lab200_unpack8(None, p, p, 2, 64, _lib.BF16, None) == 1 and L.lab200_unpack8(p, p, None, 2, 64, _lib.BF16, None) == 1
 
 
