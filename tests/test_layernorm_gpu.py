@@ -68,6 +68,16 @@ def test_many_rows(cuda_lib, m, n, dtype, gated):
     check(*inputs(m, n, dtype, torch.float32, gated, seed=1), save_8bit=True)
 
 
+@pytest.mark.parametrize("m", [149, 445, 741])
+@pytest.mark.parametrize("n", [4104, 5120, 6144, 6152, 8192])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_wide_rows(cuda_lib, m, n, dtype):
+    """Rows of which an SM has one or two teams, with a last turn that some teams have no row for."""
+    for gated in (False, True):
+        for save_8bit in (False, True):
+            check(*inputs(m, n, dtype, torch.float32, gated), save_8bit=save_8bit, what=f"gate={gated} 8bit={save_8bit} ")
+
+
 @pytest.mark.parametrize("has_w,has_b", [(False, False), (True, False), (False, True)])
 @pytest.mark.parametrize("n", [100, 1024, 1001])
 def test_without_weight_or_bias(cuda_lib, n, has_w, has_b):
