@@ -582,17 +582,22 @@ __global__ void __launch_bounds__((LN_FWD_THREADS<GATE, SAVE>)) ln_fwd_kernel(co
 // A row is a team's of T threads, V packs a thread (E = P V values), as in the forward pass, and a thread's columns are the same for
 // all rows: it sums dw and db in registers. The copies of a row's dy, x and gate (or their checkpoints) run some rows ahead, into
 // places that are each thread's own.
-constexpr int LN_BWD_THREADS = 512;  // most of a CTA
+//
+// WIDE: rows for 257 to 320 threads, in 16 bits and without a gate, have two teams to an SM in 640 threads of 96 registers, where 512 threads
+// of 128 have one. For this a row's values are not kept over its barrier but taken from the ring and worked out again behind it, and the
+// weight is in shared memory. 16384 x 5120 bf16: 92 us, 109 with one team; from checkpoints 106 and 112. fp32 160 and 156, from checkpoints
+// 177 and 166: not there.
+constexpr int LN_BWD_THREADS = 512, LN_BWD_WIDE = 640;  // most of a CTA
 constexpr int LN_BWD_SLOTS = LN_BWD_THREADS / 64 * 2 * 128;  // two halves of 16 warps' two sums for each team of several warps
 
 struct LnBwdPlan { int T, stages; LnSteps step; };
 
 // What a team reads row by row: a tensor, or (SAVED) its checkpoint.
 // PLACE: bytes from a thread's place for one pack to that for the next.
-template <int DT, int V, bool ODD, bool SAVED>
+template <int DT, int V, int LANES, bool ODD, bool SAVED>
 struct LnRows {
   using K = LnPack<DT>;
-  static constexpr int P = K::P, H = K::H, PACK = SAVED ? P : 16, UNIT = PACK / P, PLACE = LN_BWD_THREADS * PACK, BYTES = V * PLACE;
+  static constexpr int P = K::P, H = K::H, PACK = SAVED ? P : 16, UNIT = PACK / P, PLACE = LANES * PACK, BYTES = V * PLACE;
   const char *p, *base;   // the thread's first pack of the row to start; somewhere in the tensor
   const uint8_t* e_from;  // the exponents of the row after the one at hand, those of the thread's first pack (ODD: of the row)
   uint32_t at;
@@ -734,24 +739,26 @@ __device__ __forceinline__ float2 team_sum(float2 v, uint32_t slot, int t, int T
   }
 }
 
-template <int DT, int E, int G, bool ODD, bool GATE, bool SAVED>
-__global__ void __launch_bounds__(LN_BWD_THREADS) ln_bwd_kernel(const LnArgs a, const LnBwdPlan plan) {
+template <int DT, int E, int G, bool ODD, bool GATE, bool SAVED, bool WIDE = false>
+__global__ void __launch_bounds__(WIDE ? LN_BWD_WIDE : LN_BWD_THREADS) ln_bwd_kernel(const LnArgs a, const LnBwdPlan plan) {
   using K = LnPack<DT>;
   constexpr int P = K::P, H = K::H, V = E / P;
   constexpr bool FILL = G < 32;
-  // Weight and bias: in registers, or, with a gate, where these would not do: in shared memory (PLANES), or, in fp32, where that would not
-  // either, read again for each row.
-  constexpr bool PLANES = GATE && !ODD && (DT != SRMS_F32 || SAVED), AGAIN = GATE && !ODD && !PLANES, HELD = !PLANES && !AGAIN;
-  using In = LnRows<DT, V, ODD, SAVED>;
-  using Dy = LnRows<DT, V, ODD, false>;
+  static_assert(!WIDE || (G > 32 && !ODD && !GATE), "what WIDE is for");
+  // Weight and bias: in registers, or, with a gate or in WIDE, where these would not do: in shared memory (PLANES), or, in fp32 with a gate,
+  // where that would not either, read again for each row.
+  constexpr bool PLANES = WIDE || (GATE && !ODD && (DT != SRMS_F32 || SAVED)), AGAIN = GATE && !ODD && !PLANES, HELD = !PLANES && !AGAIN;
+  constexpr int LANES = WIDE ? LN_BWD_WIDE : LN_BWD_THREADS;
+  using In = LnRows<DT, V, LANES, ODD, SAVED>;
+  using Dy = LnRows<DT, V, LANES, ODD, false>;
   constexpr uint32_t STAGE = Dy::BYTES + In::BYTES * (GATE ? 2 : 1), SLOTS = G > 32 ? LN_BWD_SLOTS : 0;
   const int T = G <= 32 ? G : plan.T, team = threadIdx.x / T, t = threadIdx.x - team * T, lanes = blockDim.x, teams = lanes / T;
   const int N = a.N;
   const float inv_n = 1.f / static_cast<float>(N);
   // shared memory: the teams' slots, weight and bias, the ring
-  constexpr uint32_t PLANE = LN_BWD_THREADS * V * 16;  // four values of each pack
+  constexpr uint32_t PLANE = (WIDE ? LANES / 2 : LANES) * V * 16;  // four values of each pack
   const uint32_t slots = static_cast<uint32_t>(__cvta_generic_to_shared(ln_shared)), planes = slots + SLOTS;
-  const uint32_t ring = PLANES ? planes + 2 * (P / 4) * PLANE : planes, ring_end = plan.stages * STAGE;
+  const uint32_t ring = PLANES ? planes + (GATE ? 2 : 1) * (P / 4) * PLANE : planes, ring_end = plan.stages * STAGE;
   uint32_t slot = slots + (G > 32 ? team * 256 : 0);
   if constexpr (G > 32)
     for (int i = threadIdx.x; i < SLOTS / 4; i += lanes) asm volatile("st.shared.u32 [%0], %1;" ::"r"(slots + 4 * i), "r"(0) : "memory");
@@ -816,7 +823,7 @@ __global__ void __launch_bounds__(LN_BWD_THREADS) ln_bwd_kernel(const LnArgs a, 
   if constexpr (PLANES)
     for (int k = threadIdx.x; k < V * T; k += lanes)  // those behind the row's end too: they are multiplied by zero
 #pragma unroll
-      for (int which = 0; which < 2; ++which) {
+      for (int which = 0; which < (GATE ? 2 : 1); ++which) {
         float f[P];
         K::params(k >= npack ? nullptr : which ? a.bias : a.weight, a.wdt, a.vec_params, k, which ? 0.f : 1.f, f);
 #pragma unroll
@@ -843,6 +850,53 @@ __global__ void __launch_bounds__(LN_BWD_THREADS) ln_bwd_kernel(const LnArgs a, 
   for (int n = 0; n < most; ++n, dx += plan.step.out, dg += plan.step.out) {
     const bool live = !FILL || n < mine;
     copies_wait(plan.stages);
+    if constexpr (WIDE) {
+      const uint32_t at = out;
+      const In row_x = x;  // its exponents
+      const float r = st.y, minus_mr = -st.x * st.y;
+      // dy with the weight's factor and xh of pack i; dy alone
+      const auto take = [&](int i, f2* sv, f2* xh, f2* d) {
+        f2 wk[H];
+        const typename Dy::Words dy_words = dy.fetch(at, i);
+        const typename In::Words x_words = x.fetch(at, i);
+        weights(i, false, wk);
+        dy.template values<false>(dy_words, i, t, T, shift, 1.f, 0.f, d);
+        row_x.template values<true>(x_words, i, t, T, shift, r, minus_mr, xh);
+#pragma unroll
+        for (int j = 0; j < H; ++j) sv[j] = f2_mul(wk[j], d[j]);
+      };
+      f2 c1 = 0, c2 = 0;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        f2 sv[H], xh[H], d[H];
+        take(i, sv, xh, d);
+#pragma unroll
+        for (int j = 0; j < H; ++j) {
+          db[i][j] = f2_add(db[i][j], d[j]);
+          dw[i][j] = f2_fma(d[j], xh[j], dw[i][j]);
+          c1 = f2_add(c1, sv[j]);
+          c2 = f2_fma(sv[j], xh[j], c2);
+        }
+      }
+      out = out + STAGE == ring_end ? 0 : out + STAGE;
+      start(n + plan.stages - 1);
+      start_small(n + 1);
+      const float2 c = team_sum<G>(make_float2(f2_sum(c1), f2_sum(c2)), slot, t, T, team);
+      slot = slots + team * 256 + ((n & 1) ? 0 : 128);
+      const float by = -inv_n * r;
+      const f2 rr = f2_all(r), k1 = f2_all(c.x * by), k2 = f2_all(c.y * by);
+      if (a.dx) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          f2 sv[H], xh[H], d[H];
+          take(i, sv, xh, d);
+#pragma unroll
+          for (int j = 0; j < H; ++j) sv[j] = f2_fma(sv[j], rr, f2_fma(xh[j], k2, k1));
+          if (t + i * T < npack) K::store(dx + i * T * 16, sv);
+        }
+      }
+      continue;
+    }
     f2 xh[V][H], s[V][H];  // s: dy, then with the gate's factor, then with the weight's
     typename Dy::Words dy_words[V];
     typename In::Words x_words[V], g_words[GATE ? V : 1];

@@ -126,7 +126,7 @@ cudaError_t ln_fwd(const LnArgs& a, LnPlace at) {
   return ln_fwd_team<DT, 4, 64, false>(a, at, team(npack, 4));
 }
 
-struct LnBwdLaunch { LnBwdPlan plan; LnRowKind kind; int G, cta; size_t shared; int parts; };
+struct LnBwdLaunch { LnBwdPlan plan; LnRowKind kind; bool wide; int G, cta; size_t shared; int parts; };
 
 // False: no kernel that keeps rows in registers takes the call.
 template <int DT>
@@ -141,11 +141,14 @@ bool ln_bwd_plan(const LnArgs& a, LnPlace at, LnBwdLaunch* l) {
   const int E = odd && gate ? 8 : 16, V = E / K::P;
   if (npack > LN_BWD_THREADS * V) return false;
   l->G = npack <= 2 * V ? 2 : npack <= 4 * V ? 4 : npack <= 8 * V ? 8 : npack <= 16 * V ? 16 : npack <= 32 * V ? 32 : 64;
-  const int T = l->G <= 32 ? l->G : team(E), teams = LN_BWD_THREADS / T;
+  const int T = l->G <= 32 ? l->G : team(E);
+  l->wide = K::P == 8 && !odd && !gate && T > LN_BWD_THREADS / 2 && T <= LN_BWD_WIDE / 2;
+  const int lanes = l->wide ? LN_BWD_WIDE : LN_BWD_THREADS, teams = lanes / T;
   l->cta = teams * T;
-  const size_t in = static_cast<size_t>(V) * LN_BWD_THREADS * (saved ? K::P : 16), stage = static_cast<size_t>(V) * LN_BWD_THREADS * 16 + in * (gate ? 2 : 1);
+  const size_t in = static_cast<size_t>(V) * lanes * (saved ? K::P : 16), stage = static_cast<size_t>(V) * lanes * 16 + in * (gate ? 2 : 1);
   // the kernel's slots and planes
-  const size_t fixed = (l->G > 32 ? LN_BWD_SLOTS : 0) + (gate && !odd && (K::P == 8 || saved) ? static_cast<size_t>(2 * K::P / 4) * LN_BWD_THREADS * V * 16 : 0);
+  const size_t planes = l->wide ? lanes / 2 : gate && !odd && (K::P == 8 || saved) ? 2 * lanes : 0;
+  const size_t fixed = (l->G > 32 ? LN_BWD_SLOTS : 0) + planes * (K::P / 4) * V * 16;
   const int units = l->cta / (l->G <= 32 ? 32 : T);
   const size_t sums = odd ? static_cast<size_t>(teams) * a.N * 4 : static_cast<size_t>(units - 1) * E * T * 4;
   constexpr size_t room = LN_SHARED - LN_STATIC;
@@ -167,6 +170,9 @@ cudaError_t ln_bwd_team(const LnArgs& a, LnPlace at, const LnBwdLaunch& l) {
   constexpr int E = 16, EG = ODD ? 8 : 16;
   if (gate) return saved ? ln_launch<ln_bwd_kernel<DT, EG, G, ODD, true, true>>(l.parts, l.cta, l.shared, at, a, l.plan)
                          : ln_launch<ln_bwd_kernel<DT, EG, G, ODD, true, false>>(l.parts, l.cta, l.shared, at, a, l.plan);
+  if constexpr (G > 32 && !ODD && LnPack<DT>::P == 8)
+    if (l.wide) return saved ? ln_launch<ln_bwd_kernel<DT, E, G, false, false, true, true>>(l.parts, l.cta, l.shared, at, a, l.plan)
+                             : ln_launch<ln_bwd_kernel<DT, E, G, false, false, false, true>>(l.parts, l.cta, l.shared, at, a, l.plan);
   return saved ? ln_launch<ln_bwd_kernel<DT, E, G, ODD, false, true>>(l.parts, l.cta, l.shared, at, a, l.plan)
                : ln_launch<ln_bwd_kernel<DT, E, G, ODD, false, false>>(l.parts, l.cta, l.shared, at, a, l.plan);
 }
