@@ -256,12 +256,6 @@ __device__ __forceinline__ float4 shared_f4(uint32_t at) {
   const uint4 v = shared16(at);
   return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
 }
-__device__ __forceinline__ float2 shared_f2(uint32_t at) {
-  float2 v;
-  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
-  return v;
-}
-__device__ __forceinline__ void shared_put(uint32_t at, float2 v) { asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(v.x), "f"(v.y) : "memory"); }
 __device__ __forceinline__ void shared_put(uint32_t at, float4 v) {
   asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }

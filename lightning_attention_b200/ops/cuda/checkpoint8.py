@@ -9,6 +9,12 @@ import torch
 from ... import _lib
 
 GROUP = 32
+MAX_ROW = 1 << 30  # values of a row: the kernels count within one in 32 bits
+
+
+def check_row(t, what):
+    if t.dim() < 1 or not 1 <= t.shape[-1] <= MAX_ROW:
+        raise RuntimeError(f"{what} of at least one value and at most 2^30, got shape {tuple(t.shape)}")
 
 
 def rows(t, N):
@@ -57,10 +63,9 @@ def pack_8bit(x):
         r = _lib.host().pack8(x)
         if r is not None:
             return r
+    check_row(x, "pack_8bit takes a tensor with a last dimension")
     _lib.require_cuda(x)
     dt = _lib.dtype_code(x.dtype)
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise RuntimeError(f"pack_8bit takes a tensor with a last dimension of at least one value, got shape {tuple(x.shape)}")
     N = x.shape[-1]
     codes, scales = empty_checkpoint(x.shape, x.device)
     x, ld = rows(x.detach(), N)
@@ -77,6 +82,8 @@ def unpack_8bit(codes, scales, dtype=torch.bfloat16):
         y = _lib.host().unpack8(codes, scales, dt)
         if y is not None:
             return y
+    if codes.dim() > 0 and codes.shape[-1] > MAX_ROW:
+        raise RuntimeError(f"unpack_8bit takes codes with a last dimension of at most 2^30, got shape {tuple(codes.shape)}")
     _lib.require_cuda(codes, scales)
     if codes.dim() < 1 or codes.shape[-1] < 1 or not checkpoint_fits(codes, scales, codes.shape, codes.device):
         raise RuntimeError("expected int8 codes and uint8 scales with one byte for each 32 codes of the last dimension, on one device; got "

@@ -6,14 +6,13 @@ With `save_8bit` the backward pass keeps x (and the gate) as 8-bit checkpoints, 
 import torch
 
 from ... import _lib
-from .checkpoint8 import checkpoint_fits, differentiable_once, empty_checkpoint, packed_rows
+from .checkpoint8 import check_row, checkpoint_fits, differentiable_once, empty_checkpoint, packed_rows
 
 
 def _check(x, gate, weight, bias, eps):
+    check_row(x, "layer norm takes rows")
     _lib.require_cuda(x, gate, weight, bias)
     _lib.dtype_code(x.dtype)
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise RuntimeError(f"layer norm takes rows of at least one value, got shape {tuple(x.shape)}")
     if gate is not None and (gate.shape != x.shape or gate.dtype != x.dtype or gate.device != x.device):
         raise RuntimeError(f"gate must match x in shape, dtype and device; got {tuple(gate.shape)} {gate.dtype} {gate.device} vs "
                            f"{tuple(x.shape)} {x.dtype} {x.device}")

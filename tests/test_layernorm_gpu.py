@@ -364,6 +364,24 @@ def test_refusals(cuda_lib):
         la.layer_norm(x.double())
 
 
+def test_rows_past_what_the_kernels_count_are_refused(cuda_lib):
+    x = torch.zeros(1, device=DEV).expand(2, (1 << 32) + 64)
+    for call in (lambda: la.layer_norm(x), lambda: la.layer_norm_sigmoid_gate(x, x), lambda: la.pack_8bit(x)):
+        with pytest.raises(RuntimeError, match="at most 2\\^30"):
+            call()
+
+
+@pytest.mark.parametrize("m,n", [(300, 1024), (9, 1001), (40, 5120)])
+def test_one_tensor_in_two_places(cuda_lib, m, n):
+    """x as its own gate, and the weight as the bias: gradients add up; a gradient that is the input itself."""
+    for save_8bit in (False, True):
+        x, _, w, _, _ = inputs(m, n, torch.float32)
+        both = fwd_bwd(x, x.detach().clone().requires_grad_(), w, w.detach().clone().requires_grad_(), x.detach(), save_8bit)
+        y = call(x, x, w, w, save_8bit)
+        dx, dw = torch.autograd.grad(y, (x, w), x.detach())
+        assert torch.equal(y.detach(), both["y"]) and torch.equal(dx, both["dx"] + both["dgate"]) and torch.equal(dw, both["dw"] + both["db"])
+
+
 def test_side_stream_and_two_threads(cuda_lib):
     args = inputs(700, 1024, torch.bfloat16, torch.float32, True)
     want = fwd_bwd(*args)

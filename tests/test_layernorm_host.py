@@ -40,6 +40,16 @@ def test_cpu_tensors_are_refused():
         la.lightning_attn_func(q, q, q, torch.zeros(2), save_8bit=True)
 
 
+@pytest.mark.parametrize("n", [(1 << 30) + 1, (1 << 32) + 64])
+def test_rows_past_what_the_kernels_count_are_refused(n):
+    """Lengths that a 32-bit count would cut short, of views that hold one value."""
+    x, codes = torch.zeros(1).expand(2, n), torch.zeros(1, dtype=torch.int8).expand(2, n)
+    scales = torch.zeros(1, dtype=torch.uint8).expand(2, -(-n // 32))
+    for call in (lambda: la.layer_norm(x), lambda: la.layer_norm_sigmoid_gate(x, x), lambda: la.pack_8bit(x), lambda: la.unpack_8bit(codes, scales)):
+        with pytest.raises(RuntimeError, match="at most 2\\^30"):
+            call()
+
+
 def test_layernorm_fwd_argument_validation():
     L, p = _lib.lib(), _p()
 
