@@ -58,9 +58,10 @@ PkRows pk_rows(long long M, long long N, int P, bool contiguous) {
   r.items = M * per_row;
   r.per_row = M == 1 ? 0 : static_cast<int>(per_row);
   // rows that fill their last item well are left to warps, whose place costs less (20000 x 1000 in 12 us
-  // against 15; 27408 x 312 in 14 against 6, a warp having 40 packs for 128)
-  if (P && M > 1 && units * 10 < per_row * per * 9 && M * units <= (1ll << 31) - per) {
-    // n / d = umulhi(n, ceil(2^(31 + l) / d)) >> (l - 1) for n < 2^31 and 2^(l - 1) < d <= 2^l: the factor is too large by less
+  // against 15; 27408 x 312 in 14 against 6, a warp having 40 packs for 128; value by value 27965 x 562
+  // in 27 us against 35; 374506 x 51 in 117 against 51, a warp having 2 groups for 8)
+  if (M > 1 && units * 10 < per_row * per * (P ? 9 : 6) && M * units <= (1ll << 31) - per) {
+    // n / d = umulhi(n, ceil(2^(31 + l) / d)) >> (l - 1) for n < 2^31, d > 1 and 2^(l - 1) < d <= 2^l: the factor is too large by less
     // than d / 2^(31 + l), which n times stays below 1 / d
     int l = 1;
     while ((1ll << l) < units) ++l;
@@ -192,7 +193,8 @@ int lab200_pack8(const void* x, long long ldx, void* codes, void* scales, long l
   const PkRows r = pk_rows(M, N, packs ? 16 / esz : 0, ldx == N);
   const unsigned grid = ln_capped((r.items + 7) / 8, 16LL * place(st).sms);
 #define LAB200_PACK(DT) \
-  !packs ? pack8_any_kernel<DT, PK_U_ANY><<<grid, 256, 0, st>>>(x, ldx, c, s, N, r) \
+  !packs && r.units ? pack8_any_kernel<DT, PK_U_ANY, true><<<grid, 256, 0, st>>>(x, ldx, c, s, N, r) \
+  : !packs ? pack8_any_kernel<DT, PK_U_ANY, false><<<grid, 256, 0, st>>>(x, ldx, c, s, N, r) \
   : r.units ? pack8_kernel<DT, PK_U, true><<<grid, 256, 0, st>>>(x, ldx, c, s, r) : pack8_kernel<DT, PK_U, false><<<grid, 256, 0, st>>>(x, ldx, c, s, r)
   if (dtype == LAB200_F32) LAB200_PACK(SRMS_F32);
   else if (dtype == LAB200_F16) LAB200_PACK(SRMS_F16);
@@ -215,7 +217,8 @@ int lab200_unpack8(const void* codes, const void* scales, void* y, long long M, 
   const PkRows r = pk_rows(M, N, packs ? 16 / esz : 0, true);
   const unsigned grid = ln_capped((r.items + 7) / 8, 16LL * place(st).sms);
 #define LAB200_UNPACK(DT) \
-  !packs ? unpack8_any_kernel<DT, PK_U_ANY><<<grid, 256, 0, st>>>(c, s, y, N, r) \
+  !packs && r.units ? unpack8_any_kernel<DT, PK_U_ANY, true><<<grid, 256, 0, st>>>(c, s, y, N, r) \
+  : !packs ? unpack8_any_kernel<DT, PK_U_ANY, false><<<grid, 256, 0, st>>>(c, s, y, N, r) \
   : r.units ? unpack8_kernel<DT, PK_U, true><<<grid, 256, 0, st>>>(c, s, y, r) : unpack8_kernel<DT, PK_U, false><<<grid, 256, 0, st>>>(c, s, y, r)
   if (dtype == LAB200_F32) LAB200_UNPACK(SRMS_F32);
   else if (dtype == LAB200_F16) LAB200_UNPACK(SRMS_F16);

@@ -39,6 +39,17 @@ def test_round_trip(cuda_lib, shape, dtype):
     torch.testing.assert_close(y, want(x), rtol=0, atol=0, equal_nan=True)  # a few fp16 inputs are infinite
 
 
+@pytest.mark.parametrize("m,n", [(70001, 1), (5003, 17), (2, 51), (3001, 51), (1001, 67), (800, 99), (257, 225), (257, 257), (90, 290), (300, 562), (61, 1010)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_odd_rows(cuda_lib, m, n, dtype):
+    """Rows that packs do not divide, of 1 to 32 groups: counted over all rows, or by row; contiguous and not; nothing behind the ends."""
+    torch.manual_seed(0)
+    wide = (torch.randn(m, n + 3, device=DEV) * torch.exp(3 * torch.randn(m, n + 3, device=DEV))).to(dtype)
+    for x in (wide[:, :n].contiguous(), wide[:, 1:n + 1]):
+        _, _, y = round_trip(x)
+        torch.testing.assert_close(y, want(x), rtol=0, atol=0, equal_nan=True)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_values_at_the_border(cuda_lib, dtype):
     """Ties, groups whose largest value rounds up to 128 steps, powers of two, zeros, the largest and the smallest values of the type."""
