@@ -358,9 +358,11 @@ extern __shared__ __align__(16) char ln_shared[];
 // A row is a team's of T threads, V packs a thread: T a power of two up to 32 (several rows in a warp) or a multiple of 32. A warp
 // has the mean and the squares about it of its part of a row from shuffles; the parts are joined by the formula for the variance of
 // a union, behind the only barrier of a row. Each thread has places of its own in the ring of copies, so that it needs none.
-// Most threads of a CTA: 20 warps of up to 96 registers hide more than 16 of 128 do (32768 x 4096 bf16: 95 us, 106), but for the gated
-// norm that writes checkpoints, which spills then.
-template <bool GATE, bool SAVE> constexpr int LN_FWD_THREADS = GATE && SAVE ? 512 : 640;
+// Most threads of a CTA: 20 warps of up to 96 registers hide more than 16 of 128 do (32768 x 4096 bf16: 91 us, 100; 16384 x 5120 gated,
+// writing checkpoints: 122, 130). Gated rows of which the copies of 640 threads do not fit beside weight and bias (from 7784 values on) take 512,
+// up to 11872 values: 8192 x 8192 gated, writing checkpoints, 103 us, 403 value by value.
+// Bound by memory without a gate or checkpoints (5.9 TB/s at 32768 x 4096 bf16), else by instructions too (with both 186 us, 5.8 TB/s).
+constexpr int LN_FWD_THREADS = 640, LN_FWD_FEWER = 512;
 
 // Strides from one of a team's rows to its next, in bytes: all teams' rows at once. As arguments they cost the kernels no registers.
 struct LnSteps {
@@ -373,13 +375,13 @@ struct LnSteps {
 
 struct LnFwdPlan { int T, stages; LnSteps step; };
 
-template <int DT, int V, int G, bool ODD, bool GATE, bool SAVE>
-__global__ void __launch_bounds__((LN_FWD_THREADS<GATE, SAVE>)) ln_fwd_kernel(const LnArgs a, const LnFwdPlan plan) {
+template <int DT, int V, int G, bool ODD, bool GATE, bool SAVE, int THREADS = LN_FWD_THREADS>
+__global__ void __launch_bounds__(THREADS) ln_fwd_kernel(const LnArgs a, const LnFwdPlan plan) {
   using K = LnPack<DT>;
   constexpr int P = K::P, H = K::H;
   static_assert(!(ODD && SAVE), "groups of 32 values do not keep to the packs of odd rows");
   // of each team's warps: mean, squares, count of their part; two halves in turn. What a team does not fill has a count of zero.
-  constexpr int THREADS = (LN_FWD_THREADS<GATE, SAVE>), WARPS = THREADS / 32, TEAMS = G > 32 ? THREADS / 64 : 1;
+  constexpr int WARPS = THREADS / 32, TEAMS = G > 32 ? THREADS / 64 : 1;
   __shared__ float4 slots[TEAMS][2][WARPS];
   const int T = G <= 32 ? G : plan.T, team = threadIdx.x / T, t = threadIdx.x - team * T, lanes = blockDim.x, warp = t >> 5;
   const int N = a.N, ng = (N - 1) / PK_GROUP + 1, teams = lanes / T;

@@ -45,7 +45,7 @@ inline long long ln_even(long long ctas, long long most, int teams, int period) 
 }
 
 // Static shared memory that a kernel may have beside its dynamic part.
-constexpr int LN_STATIC = 640 / 64 * 2 * (640 / 32) * 16;
+constexpr int LN_STATIC = LN_FWD_THREADS / 64 * 2 * (LN_FWD_THREADS / 32) * 16;
 
 // KERN has had its limit of dynamic shared memory raised on the devices whose bits are set.
 template <auto KERN>
@@ -77,9 +77,12 @@ cudaError_t ln_fwd_any(const LnArgs& a, LnPlace at) {
 template <int DT, int V, int G, bool ODD>
 cudaError_t ln_fwd_team(const LnArgs& a, LnPlace at, int T) {
   const bool gate = a.gate, save = a.xcodes;
-  const int threads = gate && save ? LN_FWD_THREADS<true, true> : LN_FWD_THREADS<false, false>, teams = threads / T, cta = teams * T, stage = threads * 16 * V * (gate ? 2 : 1);
-  const size_t planes = ODD ? 0 : static_cast<size_t>(a.N) * 8;
+  constexpr bool WIDEST = G > 32 && V == 4 && !ODD;  // the kernels that may want more room than there is
   constexpr size_t room = LN_SHARED - LN_STATIC;
+  const size_t planes = ODD ? 0 : static_cast<size_t>(a.N) * 8;
+  const auto stage_of = [&](int threads) { return threads * 16 * V * (gate ? 2 : 1); };
+  const bool fewer = WIDEST && gate && planes + 2 * stage_of(LN_FWD_THREADS) > room;
+  const int threads = fewer ? LN_FWD_FEWER : LN_FWD_THREADS, teams = threads / T, cta = teams * T, stage = stage_of(threads);
   int stages = planes > room ? 0 : static_cast<int>((room - planes) / stage);
   if (stages < 2) return ln_fwd_any<DT>(a, at);
   stages = stages > 4 ? 4 : stages;
@@ -90,6 +93,9 @@ cudaError_t ln_fwd_team(const LnArgs& a, LnPlace at, int T) {
     return gate ? ln_launch<ln_fwd_kernel<DT, V, G, true, true, false>>(grid, cta, shared, at, a, plan)
                 : ln_launch<ln_fwd_kernel<DT, V, G, true, false, false>>(grid, cta, shared, at, a, plan);
   } else {
+    if constexpr (WIDEST)
+      if (fewer) return save ? ln_launch<ln_fwd_kernel<DT, V, G, false, true, true, LN_FWD_FEWER>>(grid, cta, shared, at, a, plan)
+                           : ln_launch<ln_fwd_kernel<DT, V, G, false, true, false, LN_FWD_FEWER>>(grid, cta, shared, at, a, plan);
     if (gate) return save ? ln_launch<ln_fwd_kernel<DT, V, G, false, true, true>>(grid, cta, shared, at, a, plan)
                           : ln_launch<ln_fwd_kernel<DT, V, G, false, true, false>>(grid, cta, shared, at, a, plan);
     return save ? ln_launch<ln_fwd_kernel<DT, V, G, false, false, true>>(grid, cta, shared, at, a, plan)

@@ -78,6 +78,14 @@ def test_wide_rows(cuda_lib, m, n, dtype):
             check(*inputs(m, n, dtype, torch.float32, gated), save_8bit=save_8bit, what=f"gate={gated} 8bit={save_8bit} ")
 
 
+@pytest.mark.parametrize("n", [7776, 7784, 8192, 11872, 11880, 12000])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_rows_that_fill_shared_memory(cuda_lib, n, dtype):
+    """Lengths on both sides of those at which the gated forward kernel has room for its copies."""
+    for save_8bit in (False, True):
+        check(*inputs(299, n, dtype, torch.float32, True), save_8bit=save_8bit, what=f"8bit={save_8bit} ")
+
+
 @pytest.mark.parametrize("has_w,has_b", [(False, False), (True, False), (False, True)])
 @pytest.mark.parametrize("n", [100, 1024, 1001])
 def test_without_weight_or_bias(cuda_lib, n, has_w, has_b):
