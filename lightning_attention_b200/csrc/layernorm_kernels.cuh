@@ -361,6 +361,7 @@ extern __shared__ __align__(16) char ln_shared[];
 // Most threads of a CTA: 20 warps of up to 96 registers hide more than 16 of 128 do (32768 x 4096 bf16: 91 us, 100; 16384 x 5120 gated,
 // writing checkpoints: 122, 130). Gated rows of which the copies of 640 threads do not fit beside weight and bias (from 7784 values on) take 512,
 // up to 11872 values: 8192 x 8192 gated, writing checkpoints, 103 us, 403 value by value.
+// So do fp32 rows of several warps that packs do not divide, whose weight and bias are in registers: 8192 x 1001 gated 22 us, 25 with 640 threads.
 // Bound by memory without a gate or checkpoints (5.9 TB/s at 32768 x 4096 bf16), else by instructions too (with both 186 us, 5.8 TB/s).
 constexpr int LN_FWD_THREADS = 640, LN_FWD_FEWER = 512;
 
@@ -373,7 +374,8 @@ struct LnSteps {
         codes(all_teams * a.N), scales(all_teams * ((a.N - 1) / PK_GROUP + 1)) {}
 };
 
-struct LnFwdPlan { int T, stages; LnSteps step; };
+// parts: the warps of a team of several, rounded up to 4, 8 or 16, less one.
+struct LnFwdPlan { int T, stages, parts; LnSteps step; };
 
 template <int DT, int V, int G, bool ODD, bool GATE, bool SAVE, int THREADS = LN_FWD_THREADS>
 __global__ void __launch_bounds__(THREADS) ln_fwd_kernel(const LnArgs a, const LnFwdPlan plan) {
@@ -510,21 +512,20 @@ __global__ void __launch_bounds__(THREADS) ln_fwd_kernel(const LnArgs a, const L
       float4* slot = slots[team][turn];
       if ((t & 31) == 0) slot[warp] = make_float4(m + mean, squares, fcount, 0.f);
       asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(T) : "memory");
-      float total = 0.f, both = 0.f;
-      constexpr int AT_ONCE = SAVE ? 4 : 2;  // without checkpoints, four spill
-      const auto join = [&](int from, int to) {
-#pragma unroll AT_ONCE
-        for (int w = from; w < to; ++w) {
-          const float d = slot[w].x - m, zd = slot[w].z * d;
-          total += zd;
-          both += fmaf(zd, d, slot[w].y);
-        }
+      // A lane takes a part. The row's mean first, counted from the first part's, then the squares about it: a sum of positive terms, so that a
+      // short part far from the rest (a last warp of four values, outliers) cancels nothing, and all warps get the same mean and spread.
+      const float4 part = slot[t & plan.parts];
+      const float ref = slot[0].x;
+      const auto over_parts = [&](float s) {
+        s += __shfl_xor_sync(0xffffffffu, s, 1);
+        s += __shfl_xor_sync(0xffffffffu, s, 2);
+        if (plan.parts > 3) s += __shfl_xor_sync(0xffffffffu, s, 4);
+        if (plan.parts > 7) s += __shfl_xor_sync(0xffffffffu, s, 8);
+        return s;
       };
-      join(0, 4);
-      if (T > 128) join(4, 8);
-      if (T > 256) join(8, WARPS);
-      mean = total * inv_n;
-      squares = fmaf(-mean, total, both);
+      const float from_ref = over_parts(part.z * (part.x - ref)) * inv_n, d = part.x - ref - from_ref;
+      squares = over_parts(fmaf(part.z * d, d, part.y));
+      mean = ref - m + from_ref;
       turn ^= 1;
     }
     squares *= inv_n;

@@ -78,20 +78,21 @@ template <int DT, int V, int G, bool ODD>
 cudaError_t ln_fwd_team(const LnArgs& a, LnPlace at, int T) {
   const bool gate = a.gate, save = a.xcodes;
   constexpr bool WIDEST = G > 32 && V == 4 && !ODD;  // the kernels that may want more room than there is
+  constexpr int MOST = ODD && G > 32 && DT == SRMS_F32 ? LN_FWD_FEWER : LN_FWD_THREADS;
   constexpr size_t room = LN_SHARED - LN_STATIC;
   const size_t planes = ODD ? 0 : static_cast<size_t>(a.N) * 8;
   const auto stage_of = [&](int threads) { return threads * 16 * V * (gate ? 2 : 1); };
   const bool fewer = WIDEST && gate && planes + 2 * stage_of(LN_FWD_THREADS) > room;
-  const int threads = fewer ? LN_FWD_FEWER : LN_FWD_THREADS, teams = threads / T, cta = teams * T, stage = stage_of(threads);
+  const int threads = fewer ? LN_FWD_FEWER : MOST, teams = threads / T, cta = teams * T, stage = stage_of(threads);
   int stages = planes > room ? 0 : static_cast<int>((room - planes) / stage);
   if (stages < 2) return ln_fwd_any<DT>(a, at);
   stages = stages > 4 ? 4 : stages;
   const size_t shared = planes + static_cast<size_t>(stages) * stage;
   const unsigned grid = static_cast<unsigned>(ln_even((a.M + teams - 1) / teams, at.sms, teams, ODD ? ln_period(a.N, LnPack<DT>::P) : 1));
-  const LnFwdPlan plan{T, stages, LnSteps(a, LnPack<DT>::ESZ, static_cast<long long>(grid) * teams)};
+  const LnFwdPlan plan{T, stages, T > 256 ? 15 : T > 128 ? 7 : 3, LnSteps(a, LnPack<DT>::ESZ, static_cast<long long>(grid) * teams)};
   if constexpr (ODD) {
-    return gate ? ln_launch<ln_fwd_kernel<DT, V, G, true, true, false>>(grid, cta, shared, at, a, plan)
-                : ln_launch<ln_fwd_kernel<DT, V, G, true, false, false>>(grid, cta, shared, at, a, plan);
+    return gate ? ln_launch<ln_fwd_kernel<DT, V, G, true, true, false, MOST>>(grid, cta, shared, at, a, plan)
+                : ln_launch<ln_fwd_kernel<DT, V, G, true, false, false, MOST>>(grid, cta, shared, at, a, plan);
   } else {
     if constexpr (WIDEST)
       if (fewer) return save ? ln_launch<ln_fwd_kernel<DT, V, G, false, true, true, LN_FWD_FEWER>>(grid, cta, shared, at, a, plan)
