@@ -350,20 +350,31 @@ bool row_type(const Tensor& x) {
   const auto t = x.scalar_type();
   return t == at::kFloat || t == at::kHalf || t == at::kBFloat16;
 }
-// Rows that are read in place: a contiguous tensor, or a matrix of any row stride.
-bool rows_in_place(const Tensor& x) {
-  return x.dim() >= 1 && x.numel() > 0 && x.size(-1) <= (1 << 30) &&
-         (x.is_contiguous() || (x.dim() == 2 && x.stride(1) == 1 && (x.size(0) == 1 || x.stride(0) >= x.size(1))));
+// The elements from one row (of the last dimension) to the next where all rows are so many apart: those of a contiguous tensor, or of a
+// slice of one along that dimension, whatever the number of leading dimensions. Else -1.
+int64_t row_stride(const Tensor& x) {
+  const int64_t N = x.size(-1);
+  if (x.is_contiguous()) return N;
+  if (N > 1 && x.stride(-1) != 1) return -1;
+  int64_t ld = -1, next = 0;  // next: the stride of a dimension that goes on where the ones after it end
+  for (int64_t i = x.dim() - 2; i >= 0; --i) {
+    if (x.size(i) == 1) continue;
+    if (ld >= 0 && x.stride(i) != next) return -1;
+    if (ld < 0) ld = x.stride(i);
+    next = x.stride(i) * x.size(i);
+  }
+  return ld < 0 ? N : ld >= N ? ld : -1;
 }
-struct Rows {
+bool rows_in_place(const Tensor& x) { return x.dim() >= 1 && x.numel() > 0 && x.size(-1) <= (1 << 30) && row_stride(x) > 0; }
+struct Rows {  // of a tensor with a row stride
   int64_t N, M, ld;
-  explicit Rows(const Tensor& x) : N(x.size(-1)), M(x.numel() / N), ld(!x.is_contiguous() && M > 1 ? x.stride(0) : N) {}
+  explicit Rows(const Tensor& x) : N(x.size(-1)), M(x.numel() / N), ld(row_stride(x)) {}
 };
 // Rows that the layer norms' fast kernels read: of a contiguous tensor that begins on 16 bytes, or whole packs of 16 bytes. Others are
 // copied, which costs less than reading them value by value (32768 x 4096 bf16: 230 us for both passes, 1040 value by value).
 Tensor to_rows(const Tensor& x) {
-  const bool packs = x.numel() > 0 && (x.size(-1) * x.element_size()) % 16 == 0 && x.dim() == 2 && (x.stride(0) * x.element_size()) % 16 == 0;
-  if (rows_in_place(x) && aligned16(x) && (x.is_contiguous() || packs)) return x;
+  const auto packs = [&] { return (x.size(-1) * x.element_size()) % 16 == 0 && (row_stride(x) * x.element_size()) % 16 == 0; };
+  if (rows_in_place(x) && aligned16(x) && (x.is_contiguous() || packs())) return x;
   return x.is_contiguous() ? x.clone() : x.contiguous();
 }
 int64_t groups(int64_t N) { return (N + 31) / 32; }
