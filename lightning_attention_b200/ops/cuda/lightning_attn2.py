@@ -325,9 +325,30 @@ class LightningAttention2NoDecay(torch.autograd.Function):
         return _bwd(q, k, v, None, do, bnhd=ctx.bnhd, kept=kept)
 
 
+MAX_WIDTH = 256  # largest d and e the kernels take in one piece
+
+
+def _pieces(t):
+    """`t` in slices of its last dimension that the kernels take."""
+    w = t.shape[-1]
+    return [t] if w <= MAX_WIDTH else [t[..., lo:lo + MAX_WIDTH].contiguous() for lo in range(0, w, MAX_WIDTH)]
+
+
+def _joined(pieces):
+    return pieces[0] if len(pieces) == 1 else torch.cat(pieces, dim=-1)
+
+
+def _added(total, t):
+    return t if total is None else total.add_(t)
+
+
 class LightningAttention2Saved8(torch.autograd.Function):
     """The same with q, k, v kept for the backward pass as 8-bit checkpoints (checkpoint8.py); s None: no decay. The forward pass is that
-    of the classes above; the gradients are theirs at the checkpoints' values, chunk states included, which are computed from those."""
+    of the classes above; the gradients are theirs at the checkpoints' values, chunk states included, which are computed from those.
+
+    d and e past MAX_WIDTH run as slices in here, and not as calls of their own that would each keep q and k (or v) again. Their
+    partial sums (o over slices of d, dv too; dq and dk over slices of e) are added in the tensors' type and in the order in which autograd
+    adds those of the call without checkpoints, so that both give the same."""
 
     @staticmethod
     def forward(ctx, q, k, v, s):
@@ -335,12 +356,19 @@ class LightningAttention2Saved8(torch.autograd.Function):
         bnhd = _use_bnhd(q, k, v)
         q, k, v = (_to_layout(t, bnhd) for t in (q, k, v))
         s = None if s is None else s.contiguous()
-        o = _fwd(q, k, v, _slopes_arg(s, q.shape[1], q.device), bnhd=bnhd)
+        sl = _slopes_arg(s, q.shape[1], q.device)
+        qs, ks = _pieces(q), _pieces(k)
+        os = []
+        for v1 in _pieces(v):
+            o = None
+            for q1, k1 in zip(qs, ks):
+                o = _added(o, _fwd(q1, k1, v1, sl, bnhd=bnhd))
+            os.append(o)
         # in the order of the memory, so that groups of 32 lie in one token's features
         packed = [pack_8bit(t.transpose(1, 2) if bnhd else t) for t in (q, k, v)]
         ctx.save_for_backward(s, *(p for pair in packed for p in pair))
         ctx.info = (q.dtype, bnhd, [tuple(p[0].shape) for p in packed])
-        return o
+        return _joined(os)
 
     @staticmethod
     def backward(ctx, do):
@@ -353,7 +381,16 @@ class LightningAttention2Saved8(torch.autograd.Function):
         q, k, v = (unpack_8bit(c, sc, dtype) for c, sc in pairs)
         if bnhd:
             q, k, v = (t.transpose(1, 2) for t in (q, k, v))
-        return _bwd(q, k, v, _slopes_arg(s, q.shape[1], q.device), _to_layout(do, bnhd), bnhd=bnhd) + (None,)
+        sl = _slopes_arg(s, q.shape[1], q.device)
+        qs, ks = _pieces(q), _pieces(k)
+        dqs, dks, dvs = [None] * len(qs), [None] * len(qs), []
+        for v1, do1 in reversed(list(zip(_pieces(v), _pieces(_to_layout(do, bnhd))))):
+            dv = None
+            for i in reversed(range(len(qs))):
+                dq1, dk1, dv1 = _bwd(qs[i], ks[i], v1, sl, do1, bnhd=bnhd)
+                dqs[i], dks[i], dv = _added(dqs[i], dq1), _added(dks[i], dk1), _added(dv, dv1)
+            dvs.insert(0, dv)
+        return _joined(dqs), _joined(dks), _joined(dvs), None
 
 
 def lightning_attn_prefill(q, k, v, s=None, kv_state=None):
@@ -406,14 +443,14 @@ def lightning_attn_decode(q, k, v, s, kv_state):
     return o.unsqueeze(2) if squeeze else o
 
 
-def _backward_can_follow(*tensors):
+def backward_can_follow(*tensors):
     return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
 
 
 def lightning_attn2(q, k, v, s, save_8bit=False):
     """LightningAttention2 through the native call path where the call has the common form, else through the class. save_8bit: the
     backward pass keeps q, k, v as 8-bit checkpoints (`pack_8bit`) and gives the gradients at their values."""
-    if save_8bit and _backward_can_follow(q, k, v):
+    if save_8bit and backward_can_follow(q, k, v):
         return LightningAttention2Saved8.apply(q, k, v, s)
     if s is not None and not torch.compiler.is_compiling():
         o = _lib.host().attn(q, k, v, s)
@@ -424,7 +461,7 @@ def lightning_attn2(q, k, v, s, save_8bit=False):
 
 def lightning_attn2_no_decay(q, k, v, save_8bit=False):
     """LightningAttention2NoDecay, the same way."""
-    if save_8bit and _backward_can_follow(q, k, v):
+    if save_8bit and backward_can_follow(q, k, v):
         return LightningAttention2Saved8.apply(q, k, v, None)
     if not torch.compiler.is_compiling():
         o = _lib.host().attn_no_decay(q, k, v)

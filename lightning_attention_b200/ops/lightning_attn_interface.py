@@ -12,8 +12,8 @@ import torch
 import torch.nn.functional as F
 
 from .cuda import lightning_attn2, lightning_attn2_no_decay
-
-_MAX_D = 256  # largest d (and e) the kernels take in one piece
+from .cuda.lightning_attn2 import MAX_WIDTH as _MAX_D
+from .cuda.lightning_attn2 import backward_can_follow
 
 
 def is_support(dim):
@@ -63,9 +63,11 @@ def lightning_attn_func(q, k, v, s=None, variant="chunk_loop", save_8bit=False):
             o1 = o1 + fn(q[..., start:start + _MAX_D], k[..., start:start + _MAX_D], v1)
         return o1
 
+    if save_8bit and backward_can_follow(q, k, v):
+        o = fn(q, k, v)  # of any width: cut inside, so that each of q, k, v is kept once
     # Output columns are independent of each other: e > 256, which the backward kernels do not take in one piece (dq
     # contracts over e), runs as column slices of v whose outputs are concatenated; autograd sums their dq and dk.
-    if v.shape[-1] > _MAX_D:
+    elif v.shape[-1] > _MAX_D:
         o = torch.cat([over_d(v[..., start:start + _MAX_D]) for start in range(0, v.shape[-1], _MAX_D)], dim=-1)
     else:
         o = over_d(v)
