@@ -74,8 +74,11 @@ __device__ __forceinline__ float ln_saved(const void* p, long long ld, const int
 }
 
 // ---- rows of any length, stride and alignment: a CTA per row, element by element, each row read again for each sum ----------
-// For rows past what teams hold (8192 values and more) and for C callers' rows that the Python operators would copy. Bound by
-// instructions: 32768 x 4096 bf16 in 1040 us, both passes.
+// For C callers' rows that the Python operators would copy, and for rows past what teams hold:
+//   rows that packs divide      forward 16384 values of 16 bits (gated 11872: shared memory), 8192 of 32; backward 8192
+//   rows that packs do not      8185 of 16 bits, 8189 of 32; gated, backward, 4089 and 4093: weight and bias of columns that each team has for
+//                               itself stay in registers beside the two sums, and with 16 values a thread they do not fit
+// Bound by instructions: 32768 x 4096 bf16 in 1040 us, both passes.
 template <int DT>
 __global__ void __launch_bounds__(256) ln_fwd_any_kernel(const LnArgs a) {
   using E = SrmsElem<DT>;
