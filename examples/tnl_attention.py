@@ -10,7 +10,7 @@ differences in how the attention op is fed and drained:
   reference's example has, `layer_norm_sigmoid_gate`.
 
 `save_8bit=True` keeps what the attention op and (with `norm="layer"`) the norm and gate need for the backward pass as 8-bit checkpoints:
-half the memory of those activations, gradients at the checkpoints' values. `fused=False` runs the same arithmetic the unfused way (contiguous copies, separate norm, sigmoid and multiply), which
+half the memory of those activations, gradients from the checkpoints' values. `fused=False` runs the same arithmetic the unfused way (contiguous copies, separate norm, sigmoid and multiply), which
 is what the tests compare against.
 """
 import torch

@@ -281,9 +281,9 @@ size_t lab200_layernorm_bwd_workspace_bytes(long long M, int N);
 
 /*
  * Gradients of the above. x (and gate) are given as tensors, or, with x (and gate) NULL, as the checkpoints that the forward pass
- * wrote. dy: rows of lddy; dx, dgate: (M, N) contiguous of `dtype`; dweight, dbias: N values of `wdtype`. Each of the four may
- * be NULL where it is not wanted. bias only matters with a gate. Deterministic: sums over rows go through partial sums in
- * `workspace` (16-byte aligned) in a fixed order.
+ * wrote; stats are those of the forward pass either way, of x itself. dy: rows of lddy; dx, dgate: (M, N) contiguous of `dtype`;
+ * dweight, dbias: N values of `wdtype`. Each of the four may be NULL where it is not wanted. bias only matters with a gate.
+ * Deterministic: sums over rows go through partial sums in `workspace` (16-byte aligned) in a fixed order.
  */
 int lab200_layernorm_bwd(const void* x, long long ldx, const void* gate, long long ldg, const void* xcodes, const void* xscales,
                          const void* gcodes, const void* gscales, const float* stats, const void* dy, long long lddy,

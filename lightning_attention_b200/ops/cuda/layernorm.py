@@ -1,7 +1,7 @@
 """Layer norm with weight and bias, and the same followed by a sigmoid gate, as torch.autograd.Functions backed by liblightning_b200.so.
 
 The norm of the reference's example caller is nn.LayerNorm, its output times a sigmoid gate (examples/module/tnl_attn.py:66-69).
-With `save_8bit` the backward pass keeps x (and the gate) as 8-bit checkpoints, which the forward kernel writes beside y.
+With `save_8bit` the backward pass keeps x (and the gate) as 8-bit checkpoints, which the forward kernel writes beside y and the row statistics.
 """
 import torch
 
@@ -114,13 +114,14 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, save_8bit=False):
 
     x: bf16, fp16 or fp32, any strides; weight, bias: (N,) of x's dtype or fp32, one dtype for both. Statistics and all sums are
     fp32. Differentiable once, in x, weight and bias; gradients are the same every time. save_8bit: the backward pass keeps x as an
-    8-bit checkpoint (`pack_8bit`) in place of the tensor, and gives the gradients at the checkpoint's values."""
+    8-bit checkpoint (`pack_8bit`) in place of the tensor, and each row's mean and 1 / sqrt(var + eps) as they were in the forward pass:
+    it takes x from the checkpoint in the gradients' formulas and the statistics of x itself, not those of the checkpoint."""
     return _apply(x, None, weight, bias, eps, save_8bit)
 
 
 def layer_norm_sigmoid_gate(x, gate, weight=None, bias=None, eps=1e-5, save_8bit=False):
     """layer_norm(x, weight, bias, eps) * sigmoid(gate) in one kernel each way; gate has x's shape and dtype. save_8bit: x and gate
-    are both kept as 8-bit checkpoints."""
+    are both kept as 8-bit checkpoints, and the row statistics of x itself."""
     if gate is None:
         raise RuntimeError("layer_norm_sigmoid_gate needs a gate; layer_norm has none")
     return _apply(x, gate, weight, bias, eps, save_8bit)
