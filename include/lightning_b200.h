@@ -292,8 +292,9 @@ int lab200_layernorm_bwd(const void* x, long long ldx, const void* gate, long lo
 
 /*
  * 8-bit checkpoint of M rows of N values (row stride ldx): each 32 consecutive values of a row, the last of a row fewer, share
- * an exponent byte E and keep a signed byte each, value = code * 2^(E - 133), off by at most half of that step; E = 255: the
- * group held an infinity or a NaN and comes back as NaN. codes: (M, N) int8; scales: (M, ceil(N / 32)) uint8, both contiguous.
+ * an exponent byte E and keep a signed byte each, value = code * 2^(E - 133), 7 <= E <= 254, off by at most half of that step (fp32
+ * values of 127.5 * 2^121 and above, which code 127 stands for, by up to one); E = 255: the group held an infinity or a NaN and
+ * comes back as NaN. codes: (M, N) int8; scales: (M, ceil(N / 32)) uint8, both contiguous.
  * Rounding is to nearest even and exact whatever the type of x. No counterpart in the reference.
  */
 int lab200_pack8(const void* x, long long ldx, void* codes, void* scales, long long M, int N, int dtype, void* stream);

@@ -3,8 +3,9 @@
 //   step = 2^(E - 133);   code = rint(x / step), in [-127, 127];   value = code * step
 //   E    = exponent field of the group's largest magnitude, one more where that would round to 128 steps; 7 <= E <= 254
 //
-// so a group's largest value is 63.5 to 127.5 steps and every value is off by at most half a step, 2^-7 of that largest value
-// (values of 127.5 * 2^121 and above, where E is at its end, come back as 127 * 2^121). The step is a power of two so that
+// so a group's largest value is 63.75 (where E is raised) to 127.5 steps and every value is off by at most half a step, 1 / 127.5 of that
+// largest value. At E's ends that bound is another: groups below 2^-120 have the step 2^-126, and their values up to half of it come back
+// as zero; values of 127.5 * 2^121 and above come back as 127 * 2^121, up to a step less. The step is a power of two so that
 // scaling is exact: a code is one rounding of the exact quotient whatever computes it, and the value it stands for is exact in
 // fp32 and bf16. A group that holds an infinity or a NaN has E = 255 and comes back as NaN.
 #pragma once

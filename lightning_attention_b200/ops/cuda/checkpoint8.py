@@ -1,8 +1,8 @@
 """8-bit activation checkpoints: pack_8bit and unpack_8bit, and what the operators with `save_8bit` use of them.
 
 32 consecutive values of the last dimension share one exponent byte and keep a signed byte each (csrc/pack8.cuh): 8.25 bits per value,
-off by at most 2^-7 of the largest of the 32. The step is a power of two, so that what a checkpoint stands for depends on its
-input alone, and is exact in fp32 and bf16.
+off by at most 1 / 127.5 of the largest of the 32 (of those below 2^-120, where steps end, by up to 2^-127). The step is a power of two, so
+that what a checkpoint stands for depends on its input alone, and is exact in fp32 and bf16.
 """
 import torch
 
