@@ -360,12 +360,12 @@ extern __shared__ __align__(16) char ln_shared[];
 // ---- forward -----------------------------------------------------------------------------------------------------------------
 // A row is a team's of T threads, V packs a thread: T a power of two up to 32 (several rows in a warp) or a multiple of 32. A warp
 // has the mean and the squares about it of its part of a row from shuffles; the parts are joined by the formula for the variance of
-// a union, behind the only barrier of a row. Each thread has places of its own in the ring of copies, so that it needs none.
+// a union, a lane to a part, behind the only barrier of a row. Each thread has places of its own in the ring of copies, so that it needs none.
 // Most threads of a CTA: 20 warps of up to 96 registers hide more than 16 of 128 do (32768 x 4096 bf16: 91 us, 100; 16384 x 5120 gated,
 // writing checkpoints: 122, 130). Gated rows of which the copies of 640 threads do not fit beside weight and bias (from 7784 values on) take 512,
 // up to 11872 values: 8192 x 8192 gated, writing checkpoints, 103 us, 403 value by value.
 // So do fp32 rows of several warps that packs do not divide, whose weight and bias are in registers: 8192 x 1001 gated 22 us, 25 with 640 threads.
-// Bound by memory without a gate or checkpoints (5.9 TB/s at 32768 x 4096 bf16), else by instructions too (with both 186 us, 5.8 TB/s).
+// Bound by memory without a gate or checkpoints (5.9 TB/s at 32768 x 4096 bf16), else by instructions too (with both 187 us, 5.8 TB/s).
 constexpr int LN_FWD_THREADS = 640, LN_FWD_FEWER = 512;
 
 // Strides from one of a team's rows to its next, in bytes: all teams' rows at once. As arguments they cost the kernels no registers.

@@ -120,8 +120,8 @@ cudaError_t ln_fwd(const LnArgs& a, LnPlace at) {
   const int npack = a.N / K::P;
   if (kind != LN_PACKS || npack > 512 * 4) return ln_fwd_any<DT>(a, at);
   // Rows of which one for each team of one pack a thread fills the GPU once or less: more threads to a row then cost less than they gain.
-  // Measured with one pack and with four, bf16: 1 x 2048 in 3.1 and 3.3 us, 296 x 2048 in 3.6 and 4.8, 888 x 2048 in 5.6 and 4.9;
-  // 888 x 768 in 3.7 and 3.9, 1184 x 768 in 4.6 and 3.9.
+  // Measured with one pack and with four, bf16, rows from memory: 1 x 2048 in 3.3 and 3.5 us, 296 x 2048 in 3.9 and 5.1, 888 x 2048 in 6.5
+  // and 5.8; 888 x 768 in 4.2 and 4.5, 1184 x 768 in 5.4 and 4.6.
   if (npack <= 512 && a.M * (npack <= 32 ? 32 : team(npack, 1)) <= at.sms * 640LL)
     return npack <= 32 ? ln_fwd_team<DT, 1, 32, false>(a, at, 32) : ln_fwd_team<DT, 1, 64, false>(a, at, team(npack, 1));
   if (npack <= K::LANES) return ln_fwd_team<DT, 1, K::LANES, false>(a, at, K::LANES);

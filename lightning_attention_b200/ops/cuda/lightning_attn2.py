@@ -358,17 +358,17 @@ class LightningAttention2Saved8(torch.autograd.Function):
         s = None if s is None else s.contiguous()
         sl = _slopes_arg(s, q.shape[1], q.device)
         qs, ks = _pieces(q), _pieces(k)
-        os = []
+        outs = []
         for v1 in _pieces(v):
             o = None
             for q1, k1 in zip(qs, ks):
                 o = _added(o, _fwd(q1, k1, v1, sl, bnhd=bnhd))
-            os.append(o)
+            outs.append(o)
         # in the order of the memory, so that groups of 32 lie in one token's features
         packed = [pack_8bit(t.transpose(1, 2) if bnhd else t) for t in (q, k, v)]
         ctx.save_for_backward(s, *(p for pair in packed for p in pair))
         ctx.info = (q.dtype, bnhd, [tuple(p[0].shape) for p in packed])
-        return _joined(os)
+        return _joined(outs)
 
     @staticmethod
     def backward(ctx, do):
